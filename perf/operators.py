@@ -16,7 +16,7 @@ TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 SIZE = {"f32": 4, "f16": 2, "bf16": 2}
 EPS = 1e-6
 FP8 = torch.float8_e4m3fn
-MIN_EXP = -100          # exponent of the scale of a block that holds zeros only
+MIN_EXP, MAX_EXP = -50, 50      # exponents of scales: a block of zeros has the smallest, values beyond 448 times the largest become that
 
 
 def listed():
@@ -230,13 +230,13 @@ def _write(s):
         m = new[:, :, None, :, None]
         amax = torch.where(m, v.abs(), 0).amax((-1, -2))
         frac, exp = torch.frexp(amax)
-        exp = torch.where(amax > 0, exp - torch.where(frac <= 0.875, 9, 8), MIN_EXP).clamp(min=MIN_EXP)
+        exp = torch.where(amax > 0, exp - torch.where(frac <= 0.875, 9, 8), MIN_EXP).clamp(MIN_EXP, MAX_EXP)
         codes, scale = (torch.cat([t, t[:1]]) for t in (codes, scale))
         had = torch.frexp(scale[ids])[1] - 1
         exp = torch.where(any_old, torch.maximum(exp, had), exp)
         was = codes[ids]
         moved = torch.ldexp(was.view(FP8).float(), (had - exp)[..., None, None])
-        put = torch.where(m, torch.ldexp(v, -exp[..., None, None]), moved).to(FP8).view(torch.uint8)
+        put = torch.where(m, torch.ldexp(v, -exp[..., None, None]).clamp(-448, 448), moved).to(FP8).view(torch.uint8)
         codes[ids] = torch.where(m | old[:, :, None, :, None], put, was)
         scale[ids] = torch.ldexp(torch.ones_like(amax), exp)
         out += [codes[:-1].view(FP8), scale[:-1]]
@@ -359,12 +359,12 @@ def _exact_write(s):
                 x = s[name][r + lo - p0:r + hi - p0].double().transpose(0, 1)                     # [heads][rows][dim]
                 amax = x.abs().amax((1, 2))
                 e = torch.ceil(torch.log2((amax / 448).clamp(min=2.0 ** MIN_EXP)))
-                e = torch.where(amax > 448 * torch.exp2(e), e + 1, torch.where(amax <= 448 * torch.exp2(e - 1), e - 1, e)).clamp(min=MIN_EXP)
+                e = torch.where(amax > 448 * torch.exp2(e), e + 1, torch.where(amax <= 448 * torch.exp2(e - 1), e - 1, e)).clamp(MIN_EXP, MAX_EXP)
                 at = lo - b * BT
                 if at:
                     e = torch.maximum(e, torch.log2(sc[blk]).round())
                     val[blk, :, :at] = _e4m3(val[blk, :, :at] * (sc[blk] / torch.exp2(e))[:, None, None])
-                val[blk, :, at:at + hi - lo] = _e4m3(x / torch.exp2(e)[:, None, None])
+                val[blk, :, at:at + hi - lo] = _e4m3((x / torch.exp2(e)[:, None, None]).clamp(-448, 448))
                 sc[blk] = torch.exp2(e)
         res[name], res[name + "_scale"] = val, sc
     return res
