@@ -35,7 +35,9 @@ int msb_init(void);
 /* Synchronises the current device and returns the device-side failure word: 0, or 1/2 when a kernel abandoned a
  * bounded wait on its shared-memory ring, 3 for an abandoned peer wait.  A non-zero word means the launch that set it
  * (and anything queued behind it) returned early with incomplete outputs; the call then also resets the library's
- * device-side scheduling counters, so that later launches start from a clean state.  The word is cleared by the call. */
+ * device-side scheduling counters, so that later launches start from a clean state.  The word is cleared by the call.
+ * 4: a batch of msb_kv8_* (or a position of msb_head_norm_rope) held a number that cannot be right; 5: msb_kv8_write met
+ * a NaN.  Those calls are complete but for the sequences, blocks, rows or values concerned, as said there. */
 int msb_device_status(void);
 
 /* Block geometry: ms::q::block_elems / block_bytes / row_bytes (src/kernels/quant_types.hpp:15-36). */
@@ -280,6 +282,66 @@ size_t msb_sparse_scratch_bytes(int total_rows_max, int heads, int D);
 int msb_sparse_decode(const float* q, const float* cs, const float* sinks, int elem_type, const void* win, int n_win,
                       const void* cache, const int* topk, int k, int heads, int D, float* out, void* scratch,
                       size_t scratch_bytes, void* stream);
+
+/* ---------------------------------------------------------------- grouped-query heads over an 8-bit cache
+ * NO COUNTERPART IN THE REFERENCE, whose attention has one K == V row of 512 dims per token (encode_sparse above): the same
+ * path for layers with ordinary key / value heads -- head norms with rotation, a paged cache in 8 bits, attention over it.
+ *
+ * RMSNorm of each query and key head and the rotation by position, one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * w ;  pairs (a, b) of dims [first, first + rot) -> (a c - b s, a s + b c)
+ * pairs are (first + 2 i, first + 2 i + 1), or with halves != 0 (first + i, first + i + rot / 2); (c, s) = cs[pos[t]][i],
+ * cs F32 [n_pos][rot / 2][2].  Rows of elem_type MSB_F32 / MSB_F16 / MSB_BF16; head h of token t at q + t * q_stride + h * D
+ * (strides in elements, >= heads * D); q_w / k_w F32[D] or NULL (all ones); out may be the input.  D a multiple of 8 up to
+ * 256, first a multiple of 8, rot of 8 (halves: of 16); rot 0 = no rotation; q_heads or k_heads may be 0.  pos: device
+ * int32[n_tokens]; a row whose position is negative is padding and is left out, one with a position >= n_pos too (device
+ * status 4). */
+int msb_head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, const float* q_w, const void* k,
+                       int k_heads, int64_t k_stride, const float* k_w, int n_tokens, int D, float eps, const float* cs,
+                       const int* pos, int n_pos, int rot, int first, int halves, void* q_out, int64_t q_out_stride,
+                       void* k_out, int64_t k_out_stride, void* stream);
+/* A cache of n_blocks blocks of `block` (16, 32, 64 or 128) tokens: codes e4m3 [n_blocks][kv_heads][block][head_dim], 16-byte
+ * aligned, head_dim 64 or 128, and a power of two of [2^-50, 2^50] for each (block, head): value = code * scale. */
+typedef struct {
+  int n_blocks, kv_heads, head_dim, block;
+  void* k; void* v;                      /* device */
+  float* k_scale; float* v_scale;        /* device F32[n_blocks][kv_heads] */
+} msb_kv8_cache;
+/* A batch of sequences.  Sequence s owns rows [seq_start[s], seq_start[s + 1]) of a call's rows: its newest tokens, which
+ * are the last ones of its kv_len[s] tokens; token p lies in block table[s][p / block].  The arrays are device memory (they
+ * may change between replays of a captured call); max_new and max_len bound the rows and tokens of any sequence.  Rows
+ * behind seq_start[n_seq] are padding: never read, never written.  A sequence whose numbers cannot be right (a start that
+ * falls or lies outside [0, n_tokens], more rows than max_new or than tokens, more tokens than max_len) is left out, and a
+ * block id outside [0, n_blocks) is a block that is not there; both set device status 4. */
+typedef struct {
+  int n_seq, n_tokens, max_new, max_len;
+  const int* seq_start;                  /* int32[n_seq + 1] */
+  const int* kv_len;                     /* int32[n_seq] */
+  const int* table;                      /* int32[n_seq][table_stride] */
+  int table_stride;
+} msb_kv8_batch;
+/* Quantises the batch's rows k, v (elem_type MSB_F32 / MSB_F16 / MSB_BF16, [kv_heads][head_dim] per row, strides in elements) into
+ * their blocks.  scale = 2^E, E the smallest of [-50, 50] with max |x| <= 448 * 2^E over the block's new values of the head
+ * (50 where none is) and, where the block holds older tokens, at least its E so far; those are then rounded again to the
+ * larger scale.  Codes are rounded to nearest even; what lies beyond becomes +-448 * 2^E, an infinity too, which does not
+ * count for the maximum; a NaN becomes 0 and sets device status 5.  A block whose first token is new starts over, whatever it held.  Rows of a block behind the sequence's
+ * last token keep their bytes and mean nothing.  No two sequences of a call may write to one block. */
+int msb_kv8_write(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, const void* k, const void* v,
+                  int64_t k_stride, int64_t v_stride, void* stream);
+/* The values of the batch's rows (the last seq_start[s + 1] - seq_start[s] tokens of each sequence) into k, v; zeros for a
+ * block that is not there. */
+int msb_kv8_read(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, void* k, void* v, int64_t k_stride,
+                 int64_t v_stride, void* stream);
+/* Attention of the batch's rows q ([heads][head_dim] per row, heads a multiple of kv_heads: query head h looks at key head
+ * h / (heads / kv_heads)) over the cache, which holds their own tokens already: the row of token p sees the tokens
+ * p - window < j <= p (window 0: all up to p) whose blocks are there.
+ *   out = sum_j exp(l_j) v_j / (sum_j exp(l_j) + exp(sinks[h])),  l_j = scale q . k_j ;  sinks F32[heads] or NULL
+ * A row that sees nothing is 0.  Codes must be finite (msb_kv8_write stores no others).  Results do
+ * not depend on the run.  scratch: msb_kv8_attn_scratch_bytes(cache, batch, heads) bytes, 16-byte aligned (enough for any
+ * window; nothing in it has to be kept or cleared); calls that overlap in time need one each.  0 = bad arguments. */
+size_t msb_kv8_attn_scratch_bytes(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int heads);
+int msb_kv8_attn(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, const void* q, int64_t q_stride,
+                 int heads, float scale, int window, const float* sinks, void* out, int64_t out_stride, void* scratch,
+                 size_t scratch_bytes, void* stream);
 
 /* ---------------------------------------------------------------- small per-token kernels between the hot-path calls
  * y = x * rsqrt(mean(x^2) + eps) * w per row (w may be NULL); strides in floats, 0 = dim -- ms::arch::encode_rmsnorm

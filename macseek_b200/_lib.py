@@ -153,3 +153,23 @@ lib.msb_sample_topk.argtypes = [_vp, _i, _i, _i, C.c_float, _vp, _vp, _vp, _vp, 
 lib.msb_log_softmax.argtypes = [_vp, _vp, _i, _i, _vp]
 lib.msb_sample_top_p.argtypes = [C.POINTER(C.c_float), C.POINTER(C.c_int), _i, C.c_float, C.c_float, C.c_float, C.c_double]
 lib.msb_copy_device.argtypes = [_vp, _vp, C.c_size_t, _vp]
+
+
+class Kv8CacheC(C.Structure):
+    _fields_ = [("n_blocks", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("block", C.c_int), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class Kv8BatchC(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("max_len", C.c_int),
+                ("seq_start", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int)]
+
+
+lib.msb_head_norm_rope.argtypes = [_i, _vp, _i, _i64, _vp, _vp, _i, _i64, _vp, _i, _i, _f, _vp, _vp, _i, _i, _i, _i, _vp, _i64,
+                                   _vp, _i64, _vp]
+lib.msb_kv8_write.argtypes = [C.POINTER(Kv8CacheC), C.POINTER(Kv8BatchC), _i, _vp, _vp, _i64, _i64, _vp]
+lib.msb_kv8_read.argtypes = [C.POINTER(Kv8CacheC), C.POINTER(Kv8BatchC), _i, _vp, _vp, _i64, _i64, _vp]
+lib.msb_kv8_attn_scratch_bytes.restype = C.c_size_t
+lib.msb_kv8_attn_scratch_bytes.argtypes = [C.POINTER(Kv8CacheC), C.POINTER(Kv8BatchC), _i]
+lib.msb_kv8_attn.argtypes = [C.POINTER(Kv8CacheC), C.POINTER(Kv8BatchC), _i, _vp, _i64, _i, _f, _i, _vp, _vp, _i64, _vp,
+                             C.c_size_t, _vp]

@@ -78,6 +78,16 @@ size_t sparse_scratch_bytes(int total_rows_max, int H, int D);
 int sparse_decode(const float* q, const float* cs, const float* sinks, int elem_type, const void* win, int n_win,
                   const void* cache, const int* topk, int k, int H, int D, float* out, void* scratch,
                   size_t scratch_bytes, cudaStream_t st);
+int head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, const float* q_w, const void* k, int k_heads,
+                   int64_t k_stride, const float* k_w, int n_tokens, int D, float eps, const float* cs, const int* pos, int n_pos, int rot,
+                   int first, int halves, void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, cudaStream_t st);
+int kv8_write(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, const void* k, const void* v, int64_t k_stride,
+              int64_t v_stride, cudaStream_t st);
+int kv8_read(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, void* k, void* v, int64_t k_stride, int64_t v_stride,
+             cudaStream_t st);
+size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, int heads);
+int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, const void* q, int64_t q_stride, int heads, float scale,
+             int window, const float* sinks, void* out, int64_t out_stride, void* scratch, size_t scratch_bytes, cudaStream_t st);
 int rmsnorm(const float* x, const float* w, float* y, int rows, int dim, float eps, int in_stride, int out_stride,
             cudaStream_t st);
 int kv_window(const float* kv, const float* norm_w, const float* cs, int actq, int D, int elem_type, void* out_row,
@@ -408,6 +418,35 @@ int msb_rmsnorm(const float* x, const float* w, float* y, int rows, int dim, flo
                 void* stream) {
   return rmsnorm(x, w, y, rows, dim, eps, in_stride, out_stride, (cudaStream_t)stream);
 }
+int msb_head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, const float* q_w, const void* k,
+                       int k_heads, int64_t k_stride, const float* k_w, int n_tokens, int D, float eps, const float* cs,
+                       const int* pos, int n_pos, int rot, int first, int halves, void* q_out, int64_t q_out_stride,
+                       void* k_out, int64_t k_out_stride, void* stream) {
+  return head_norm_rope(elem_type, q, q_heads, q_stride, q_w, k, k_heads, k_stride, k_w, n_tokens, D, eps, cs, pos, n_pos,
+                        rot, first, halves, q_out, q_out_stride, k_out, k_out_stride, (cudaStream_t)stream);
+}
+
+int msb_kv8_write(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, const void* k, const void* v,
+                  int64_t k_stride, int64_t v_stride, void* stream) {
+  return kv8_write(cache, batch, elem_type, k, v, k_stride, v_stride, (cudaStream_t)stream);
+}
+
+int msb_kv8_read(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, void* k, void* v, int64_t k_stride,
+                 int64_t v_stride, void* stream) {
+  return kv8_read(cache, batch, elem_type, k, v, k_stride, v_stride, (cudaStream_t)stream);
+}
+
+size_t msb_kv8_attn_scratch_bytes(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int heads) {
+  return kv8_attn_scratch_bytes(cache, batch, heads);
+}
+
+int msb_kv8_attn(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, const void* q, int64_t q_stride,
+                 int heads, float scale, int window, const float* sinks, void* out, int64_t out_stride, void* scratch,
+                 size_t scratch_bytes, void* stream) {
+  return kv8_attn(cache, batch, elem_type, q, q_stride, heads, scale, window, sinks, out, out_stride, scratch, scratch_bytes,
+                  (cudaStream_t)stream);
+}
+
 int msb_kv_window(const float* kv, const float* norm_w, const float* cs, int actq, int D, int elem_type, void* out_row,
                   void* stream) {
   return kv_window(kv, norm_w, cs, actq, D, elem_type, out_row, (cudaStream_t)stream);

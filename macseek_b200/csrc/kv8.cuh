@@ -1,0 +1,142 @@
+// The 8-bit key / value cache of grouped-query heads: what its kernels share.
+//   codes   [n_blocks][kv_heads][block][dim] e4m3 bytes, keys and values apart; a block holds `block` tokens of one sequence
+//   scales  [n_blocks][kv_heads] f32 powers of two, keys and values apart: value = code * scale
+//   batch   seq_start [n_seq + 1]: rows of a call's new tokens; kv_len [n_seq]: tokens of the sequence, the new ones last;
+//           table [n_seq][table_stride]: the sequence's blocks in order
+// Powers of two: a code moves from one scale to a larger one by its exponent alone, so a block whose largest value grows token by
+// token keeps its older codes' mantissas, and values and codes convert without a rounding of the scale.
+#pragma once
+#include "msb_common.cuh"
+#include "kv8_index.h"
+#include "../../include/macseek_b200.h"
+
+namespace msb {
+
+enum : int { kDevBadBatch = 4, kDevNan = 5 };    // more codes of the device failure word
+// Exponents of scales.  The attention's weights carry the value scales, so that a sum of weights spans their range as well: with 100 binades
+// a token whose weight falls below 32 bits' range is 2^-26 of the sum at most.
+constexpr int kKv8MinExp = -50, kKv8MaxExp = 50;
+
+struct Kv8Cache {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int n_blocks, heads, shift;      // block = 1 << shift tokens
+};
+struct Kv8Batch {
+  const int *seq_start, *kv_len, *table;
+  int n_seq, n_tokens, max_new, max_len, table_stride;
+};
+// checks of the two structures on the host; fills the kernels' forms
+int kv8_check(const msb_kv8_cache* c, const msb_kv8_batch* b, const char* what, Kv8Cache* cc, Kv8Batch* bb);
+// A row of `dim` elements for each of `heads` heads at p + row * stride: pointer and stride, and whether 16-byte accesses are aligned.
+int kv8_rows_check(const void* p, int64_t stride, int heads, int dim, int elem_type, const char* what, bool* vec);
+
+#ifdef __CUDACC__
+// Sequence s of the batch, or an empty one where its numbers cannot be right (recorded).
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch& b, int s, int* status) {
+  Kv8Seq q;
+  if (!kv8_seq_of(__ldg(b.seq_start + s), __ldg(b.seq_start + s + 1), __ldg(b.kv_len + s), b.n_tokens, b.max_new, b.max_len, q))
+    atomicCAS(status, 0, kDevBadBatch);
+  return q;
+}
+template <class F>
+__device__ __forceinline__ int kv8_find(int n, int x, F first) {       // by whole warps
+  return kv8_search(n, x, first, [](auto f) { return __ballot_sync(0xffffffffu, f(threadIdx.x & 31)); });
+}
+// Work item `item` (kv8_index.h) and its block's id (-1: not there).
+__device__ __forceinline__ Kv8Item kv8_item(const Kv8Batch& b, const Kv8Cache& c, int item, int* status, int& id) {
+  auto first = [&](int s) { return kv8_first_item(__ldg(b.seq_start + s), s, c.shift); };
+  const int s = kv8_find(b.n_seq, item, first);
+  const Kv8Item it = kv8_item_of(kv8_seq(b, s, status), item - first(s), c.shift);
+  id = -1;
+  if (it.n == 0) return it;
+  id = __ldg(b.table + (size_t)s * b.table_stride + it.blk);
+  if (id < 0 || id >= c.n_blocks) {
+    id = -1;
+    atomicCAS(status, 0, kDevBadBatch);
+  }
+  return it;
+}
+
+__device__ __forceinline__ float kv8_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }    // -126 <= e <= 127
+__device__ __forceinline__ int kv8_exp(float scale) {
+  return min(max((int)(__float_as_uint(scale) >> 23 & 0xFF) - 127, kKv8MinExp), kKv8MaxExp);
+}
+// two codes -> two halves (exact)
+__device__ __forceinline__ uint32_t kv8_half2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
+__device__ __forceinline__ float2 kv8_float2(uint32_t codes) {
+  const uint32_t h = kv8_half2(codes);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// four values -> four codes, nearest even, beyond the format: its largest value
+__device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+      : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+
+// eight elements of a row; vec: 16-byte aligned
+template <class T> struct Elems;
+template <> struct Elems<float> {
+  static __device__ __forceinline__ void load(const float* p, bool vec, float (&v)[8]) {
+    if (vec) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = p[i];
+    }
+  }
+  static __device__ __forceinline__ void store(float* p, bool vec, const float (&v)[8]) {
+    if (vec) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) p[i] = v[i];
+    }
+  }
+  static __device__ __forceinline__ float from(float x) { return x; }
+};
+template <class T, class T2> struct Elems16 {
+  static __device__ __forceinline__ void load(const T* p, bool vec, float (&v)[8]) {
+    if (vec) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const T2 h = *reinterpret_cast<const T2*>(&w[i]);
+        v[2 * i] = static_cast<float>(h.x); v[2 * i + 1] = static_cast<float>(h.y);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = static_cast<float>(p[i]);
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, bool vec, const float (&v)[8]) {
+    if (vec) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        T2 h;
+        h.x = from(v[2 * i]); h.y = from(v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) p[i] = from(v[i]);
+    }
+  }
+  static __device__ __forceinline__ T from(float x) { return T(x); }
+};
+template <> struct Elems<__half> : Elems16<__half, __half2> {};
+template <> struct Elems<__nv_bfloat16> : Elems16<__nv_bfloat16, __nv_bfloat162> {};
+#endif  // __CUDACC__
+
+}  // namespace msb

@@ -1,0 +1,139 @@
+"""Grouped-query heads over a paged cache in 8 bits: writing new rows, reading rows back, attention (the msb_kv8_* calls;
+no counterpart in the reference, whose attention is `attn`).  Codes are e4m3 with one power-of-two scale per block of tokens
+and head; a batch of sequences is described by device arrays, so that a captured call follows them from replay to replay."""
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .core import Enc
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}      # MSB_F32, MSB_F16, MSB_BF16
+
+
+def _want(ok, what):
+    if not ok:
+        raise _lib.MsbError(what)
+
+
+def _on_stream(e, device):
+    """The library works on the current device: it has to be the stream's and the tensors'."""
+    _want(e.stream.device == device, "tensors on %s, the stream on %s" % (device, e.stream.device))
+    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else _NO_GUARD
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *a):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+class Cache:
+    """Codes uint8 [n_blocks][kv_heads][block][head_dim] and scales F32 [n_blocks][kv_heads] of keys and of values."""
+
+    def __init__(self, n_blocks, kv_heads, head_dim, block=64, device="cuda"):
+        codes = lambda: torch.zeros(n_blocks, kv_heads, block, head_dim, dtype=torch.uint8, device=device)  # noqa: E731
+        scale = lambda: torch.ones(n_blocks, kv_heads, dtype=torch.float32, device=device)  # noqa: E731
+        self._set(codes(), codes(), scale(), scale())
+
+    @classmethod
+    def of(cls, k, v, k_scale, v_scale):
+        """Over tensors that exist."""
+        c = cls.__new__(cls)
+        c._set(k, v, k_scale, v_scale)
+        return c
+
+    def _set(self, k, v, k_scale, v_scale):
+        self.device = k.device
+        for name, t, dt, shape in (("k", k, torch.uint8, k.shape), ("v", v, torch.uint8, k.shape),
+                                   ("k_scale", k_scale, torch.float32, k.shape[:2]), ("v_scale", v_scale, torch.float32, k.shape[:2])):
+            _want(t.is_cuda and t.device == self.device, "kv8 cache: %s must be on one CUDA device" % name)
+            _want(t.dtype == dt and t.shape == shape and t.is_contiguous() and k.dim() == 4,
+                  "kv8 cache: %s must be contiguous %s %s" % (name, dt, tuple(shape)))
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_blocks, self.kv_heads, self.block, self.head_dim = k.shape
+        self.c = _lib.Kv8CacheC(self.n_blocks, self.kv_heads, self.head_dim, self.block, k.data_ptr(), v.data_ptr(),
+                                k_scale.data_ptr(), v_scale.data_ptr())
+        self.ref = C.byref(self.c)
+
+
+class Batch:
+    """seq_start int32 [n + 1], kv_len int32 [n] (new tokens included), table int32 [n][blocks]; n_tokens rows in a call's
+    tensors, at most max_new new tokens and max_len tokens in any sequence."""
+
+    def __init__(self, seq_start, kv_len, table, n_tokens, max_new, max_len):
+        n = kv_len.shape[0]
+        self.device = kv_len.device
+        for name, t, shape in (("seq_start", seq_start, (n + 1,)), ("kv_len", kv_len, (n,)), ("table", table, (n, table.shape[-1]))):
+            _want(t.is_cuda and t.device == self.device, "kv8 batch: %s must be on one CUDA device" % name)
+            _want(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(),
+                  "kv8 batch: %s must be contiguous int32 %s" % (name, shape))
+        self.seq_start, self.kv_len, self.table = seq_start, kv_len, table
+        self.n_seq, self.n_tokens, self.max_new, self.max_len = n, n_tokens, max_new, max_len
+        self.c = _lib.Kv8BatchC(n, n_tokens, max_new, max_len, seq_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
+                                table.shape[1])
+        self.ref = C.byref(self.c)
+
+
+def _rows(name, t, n_tokens, heads, dim, device):
+    """MSB type of rows [n_tokens][heads][dim] whose heads are dense (tokens may be apart)."""
+    _want(t.device == device, "%s is on %s, not on %s" % (name, t.device, device))
+    _want(tuple(t.shape) == (n_tokens, heads, dim) and t.stride(2) == 1 and (t.stride(1) == dim or heads == 1),
+          "%s must be [%d][%d][%d] with dense heads" % (name, n_tokens, heads, dim))
+    ty = DTYPES.get(t.dtype)
+    _want(ty is not None, "%s must be float32, float16 or bfloat16" % name)
+    return ty
+
+
+def _stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _kv(e, cache, batch, k, v, call):
+    dev = cache.device
+    _want(batch.device == dev, "kv8: cache and batch on different devices")
+    ty = _rows("k", k, batch.n_tokens, cache.kv_heads, cache.head_dim, dev)
+    _want(_rows("v", v, batch.n_tokens, cache.kv_heads, cache.head_dim, dev) == ty, "k and v must be of one type")
+    with _on_stream(e, dev):
+        _lib.check(call(cache.ref, batch.ref, ty, k.data_ptr(), v.data_ptr(), _stride(k), _stride(v), e.handle))
+
+
+def encode_kv8_write(e: Enc, cache: Cache, batch: Batch, k, v):
+    """New rows k, v [n_tokens][kv_heads][head_dim] into the cache."""
+    _kv(e, cache, batch, k, v, _lib.lib.msb_kv8_write)
+
+
+def encode_kv8_read(e: Enc, cache: Cache, batch: Batch, k, v):
+    """The batch's rows of the cache into k, v."""
+    _kv(e, cache, batch, k, v, _lib.lib.msb_kv8_read)
+
+
+def attn_scratch(cache: Cache, batch: Batch, heads):
+    """Scratch of encode_kv8_attn for this cache and batch (any window); calls that overlap in time need one each."""
+    with torch.cuda.device(cache.device):
+        n = _lib.lib.msb_kv8_attn_scratch_bytes(cache.ref, batch.ref, heads)
+    _want(n > 0, "kv8: " + _lib.lib.msb_last_error().decode())
+    return torch.empty(n, dtype=torch.uint8, device=cache.device)
+
+
+def encode_kv8_attn(e: Enc, cache: Cache, batch: Batch, q, out, scratch, scale=None, window=0, sinks=None):
+    """Attention of the rows q [n_tokens][heads][head_dim] over the cache, which holds their tokens already, into out
+    (scale: head_dim^-0.5 if None; window 0: everything up to the row's own token; sinks: F32 [heads] or None)."""
+    dev = cache.device
+    heads = q.shape[1]
+    ty = _rows("q", q, batch.n_tokens, heads, cache.head_dim, dev)
+    _want(_rows("out", out, batch.n_tokens, heads, cache.head_dim, dev) == ty, "q and out must be of one type")
+    _want(batch.device == dev and scratch.device == dev, "kv8: cache, batch and scratch on different devices")
+    if sinks is not None:
+        _want(sinks.device == dev and sinks.dtype == torch.float32 and tuple(sinks.shape) == (heads,) and sinks.is_contiguous(),
+              "sinks must be contiguous float32 [%d]" % heads)
+    with _on_stream(e, dev):
+        _lib.check(_lib.lib.msb_kv8_attn(cache.ref, batch.ref, ty, q.data_ptr(), _stride(q), heads,
+                                         cache.head_dim ** -0.5 if scale is None else scale, window,
+                                         None if sinks is None else sinks.data_ptr(), out.data_ptr(), _stride(out),
+                                         scratch.data_ptr(), scratch.numel() * scratch.element_size(), e.handle))

@@ -1,0 +1,348 @@
+"""Grouped-query heads over the 8-bit cache: head norms with rotation, writing, reading and attention against 64 bits."""
+import pytest
+import torch
+
+import kv8_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def enc(stream=None):
+    from macseek_b200.core import Enc
+    return Enc(stream)
+
+
+def spread(t, extra=24, shift=0):
+    """The same rows inside wider ones, `shift` elements off."""
+    n, h, d = t.shape
+    buf = torch.full((n * (h * d + extra) + shift + 8,), 7.0, dtype=t.dtype, device=t.device)
+    v = buf[shift:shift + n * (h * d + extra)].view(n, h * d + extra)[:, :h * d].unflatten(1, (h, d))
+    v.copy_(t)
+    return v, buf
+
+
+# ------------------------------------------------------------------------------------------------ head norms with rotation
+NR = [(1, 64, 8, 128, 64, 64, False, "f32"), (1, 8, 1, 64, 64, 0, True, "bf16"), (37, 32, 4, 64, 32, 0, True, "f16"), (5, 7, 3, 96, 64, 32, False, "f32"),
+      (9, 3, 1, 256, 256, 0, True, "bf16"), (2, 1, 1, 8, 8, 0, False, "f32"), (3, 5, 2, 80, 48, 16, True, "f16"), (1100, 6, 2, 128, 128, 0, True, "bf16"),
+      (4, 2, 2, 128, 0, 0, False, "f32"), (1030, 40, 8, 64, 64, 0, False, "f32"), (6, 4, 4, 192, 16, 8, True, "bf16")]
+
+
+@pytest.mark.parametrize("n,qh,kh,D,rot,first,halves,dt", NR)
+@pytest.mark.parametrize("form", ("dense", "wide", "odd", "inplace", "no weights"))
+def test_head_norm_rope(n, qh, kh, D, rot, first, halves, dt, form):
+    from macseek_b200 import attn
+    g = torch.Generator().manual_seed(n + D + rot)
+    rnd = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    q, k = (3 * rnd(n, qh, D)).to(R.DT[dt]).cuda(), (rnd(n, kh, D) * 0.01).to(R.DT[dt]).cuda()
+    q[0, 0] = 0                                                     # a head of zeros
+    qw, kw = (None, None) if form == "no weights" else ((1 + 0.3 * rnd(D)).cuda(), (1 + 0.3 * rnd(D)).cuda())
+    ang = torch.arange(50, dtype=torch.float64)[:, None] * torch.pow(1e4, -torch.arange(rot // 2) / max(rot // 2, 1))[None]
+    cs = torch.stack([ang.cos(), ang.sin()], -1).float().reshape(50, rot // 2, 2).contiguous().cuda()
+    pos = torch.randint(0, 50, (n,), generator=g, dtype=torch.int32).cuda()
+    if n > 2:
+        pos[1] = -1                                                 # padding
+    want = [R.norm_rope_ref(q, qw, 1e-6, cs, pos, first, halves), R.norm_rope_ref(k, kw, 1e-6, cs, pos, first, halves)]
+    bufs = []
+    if form in ("wide", "odd"):
+        shift = 0 if form == "wide" else 1
+        (q, _), (k, _) = spread(q, 24, shift), spread(k, 8, shift)
+        (qo, b0), (ko, b1) = spread(torch.full_like(q, 7), 16, shift), spread(torch.full_like(k, 7), 40, shift)
+        bufs = [b0, b1]
+    elif form == "inplace":
+        qo, ko = q, k
+    else:
+        qo, ko = torch.full((n, qh, D), 7.0, dtype=q.dtype, device="cuda"), torch.full((n, kh, D), 7.0, dtype=q.dtype, device="cuda")
+    kept = [qo.clone(), ko.clone()]
+    e = enc()
+    attn.encode_head_norm_rope(e, q, k, qw, kw, 1e-6, cs, pos, qo, ko, rot_first=first, halves=halves)
+    e.wait()
+    half, tiny = R.half_step(q.dtype)
+    for got, (ref, tol), was in zip((qo, ko), want, kept):
+        live = (pos >= 0)
+        assert torch.equal(got[~live], was[~live])
+        assert ((got.double() - ref).abs() <= tol * (1 + half) + half * ref.abs() + tiny)[live].all()
+    for b in bufs:                                                  # nothing between the rows is touched
+        assert int((b == 7).sum()) >= 8
+        m = torch.ones_like(b, dtype=torch.bool)
+        for t in (qo, ko):
+            if t.untyped_storage().data_ptr() == b.untyped_storage().data_ptr():
+                m.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(False)
+        assert (b[m] == 7).all()
+
+
+def test_head_norm_rope_of_one_side_and_positions_beyond_the_table():
+    from macseek_b200 import _lib, attn
+    e = enc()
+    q = torch.randn(4, 3, 64, device="cuda")
+    cs = torch.randn(10, 32, 2, device="cuda")
+    pos = torch.tensor([0, 10, -3, 9], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7)
+    attn.encode_head_norm_rope(e, q, None, None, None, 1e-6, cs, pos, out, None)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 4
+    ref, tol = R.norm_rope_ref(q, None, 1e-6, cs, pos.clamp(0, 9), 0, False)
+    for r in (0, 3):
+        assert ((out[r].double() - ref[r]).abs() <= tol[r] + ref[r].abs() * 2.0 ** -24).all()
+    assert (out[1:3] == 7).all()
+    out.fill_(7)
+    attn.encode_head_norm_rope(e, None, q, None, None, 1e-6, cs, pos.clamp(0, 9), None, out)
+    e.wait()
+    assert ((out.double() - ref).abs() <= tol + ref.abs() * 2.0 ** -24).all()
+
+
+# ------------------------------------------------------------------------------------------------ writing and reading
+WR = [([(1, 1)], 1, 64, 16), ([(1, 17), (1, 16), (1, 64), (1, 65)], 8, 128, 64), ([(5, 5), (0, 9), (64, 64), (130, 200), (1, 128)], 2, 64, 64),
+      ([(300, 1000), (16, 32), (33, 47)], 3, 128, 128), ([(17, 17)] * 40, 1, 64, 32), ([(0, 0), (2, 65), (0, 3), (63, 127)], 4, 128, 16),
+      ([(1, 1 + i) for i in range(70)], 2, 64, 16)]
+
+
+@pytest.mark.parametrize("seqs,heads,dim,block", WR)
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+def test_write_and_read(seqs, heads, dim, block, dt):
+    from macseek_b200 import kv8
+    c = R.Case(seqs, heads, dim, block, seed=len(seqs) + dim, pad=3)
+    mul = 2.0 ** torch.randint(-6, 7, (c.rows, heads, 1), generator=c.g).to(R.DT[dt]).cuda()
+    k, v = c.randn(c.rows, heads, dim, dt=dt) * mul, c.randn(c.rows, heads, dim, dt=dt)
+    v[:, 0] = 0                                                      # blocks of zeros
+    k[c.start_host[-1]:] = float("nan")                              # padding
+    k, _ = spread(k, 8 if dt == "f32" else 3)
+    want = R.write_ref(c, k, v)
+    before = [t.clone() for t in (c.k, c.v)]
+    e = enc()
+    cache, batch = c.cache(), c.batch()
+    kv8.encode_kv8_write(e, cache, batch, k, v)
+    e.wait()
+    touched = torch.zeros(c.k.shape[0], c.block, dtype=torch.bool, device="cuda")      # rows that a write may change
+    for s, (n, l) in enumerate(seqs):
+        for p in range((l - n) // block * block, l if n else 0):
+            touched[int(c.table_host[s, p // block]), p % block] = True
+    for codes, scale, was, val, sc in ((c.k, c.ks, before[0], want[0], want[1]), (c.v, c.vs, before[1], want[2], want[3])):
+        m = touched[:, None, :, None].expand_as(codes)
+        assert torch.equal(codes[~m], was[~m])
+        assert torch.equal(R.values(codes)[m], val[m])
+        assert torch.equal(scale.double().nan_to_num(-1), sc.nan_to_num(-1))
+    # the rows written, and whole sequences, read back
+    for full in (False, True):
+        if full:
+            c2 = R.Case(seqs, heads, dim, block, seed=1)
+            c2.seqs = [(l, l) for _, l in seqs]
+            import numpy as np
+            st = np.cumsum([0] + [l for _, l in seqs])
+            c2.start_host, c2.rows = [int(x) for x in st], int(st[-1]) + 2
+            c2.start = torch.tensor(st, dtype=torch.int32, device="cuda")
+            c2.max_new = c2.max_len = c.max_len
+            c2.len, c2.table, c2.table_host, c2.k, c2.v, c2.ks, c2.vs = c.len, c.table, c.table_host, c.k, c.v, c.ks, c.vs
+        else:
+            c2 = c
+        for shift in (0, 1):
+            (ko, kb), (vo, vb) = (spread(torch.full((c2.rows, heads, dim), 7.0, dtype=R.DT[dt], device="cuda"), 16, shift) for _ in range(2))
+            kv8.encode_kv8_read(e, cache, c2.batch(), ko, vo)
+            e.wait()
+            for which, out in (("k", ko), ("v", vo)):
+                for s, (n, l) in enumerate(c2.seqs):
+                    r = slice(c2.start_host[s], c2.start_host[s] + n)
+                    assert torch.equal(out[r], c2.held(s, which, l - n).transpose(0, 1).float().to(R.DT[dt]))
+                assert (out[c2.start_host[-1]:] == 7).all()
+            for b, t in ((kb, ko), (vb, vo)):
+                m = torch.ones_like(b, dtype=torch.bool)
+                m.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(False)
+                assert (b[m] == 7).all()
+
+
+def test_write_token_by_token_moves_older_codes_to_a_growing_scale():
+    from macseek_b200 import kv8
+    heads, dim, block = 2, 64, 16
+    c = R.Case([(1, 1)], heads, dim, block, seed=3)
+    e = enc()
+    cache = kv8.Cache(3, heads, dim, block)
+    c.k, c.v, c.ks, c.vs = cache.k, cache.v, cache.k_scale, cache.v_scale
+    c.table_host = torch.tensor([[2, 0, 1]])
+    c.table = c.table_host.int().cuda()
+    for p in range(40):
+        c.seqs = [(1, p + 1)]
+        c.len = torch.tensor([p + 1], dtype=torch.int32, device="cuda")
+        c.max_len = p + 1
+        x = c.randn(1, heads, dim) * 2.0 ** (p % 16 - 8)
+        want = R.write_ref(c, x, -x)
+        kv8.encode_kv8_write(e, cache, c.batch(), x, -x)
+        e.wait()
+        assert torch.equal(R.values(c.k), want[0]) and torch.equal(R.values(c.v), want[2])
+        assert torch.equal(c.ks.double(), want[1]) and torch.equal(c.vs.double(), want[3])
+
+
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+def test_write_of_ends_of_the_range(dt):
+    """Values at the border of a scale, the smallest and largest numbers, infinities; a NaN is said."""
+    from macseek_b200 import _lib, kv8
+    dim, block = 64, 16
+    big = float(torch.finfo(R.DT[dt]).max)
+    rows = torch.zeros(6 * 16, 1, dim)
+    for i, top in enumerate((448.0, 448.5 if dt == "f32" else 450.0, 2.0 ** -14, big, float("inf"), 0.875)):
+        rows[16 * i:16 * i + 16] = torch.randn(16, 1, dim, generator=torch.Generator().manual_seed(i)).clamp(-1, 1) * min(top, big) * 0.5
+        rows[16 * i + 3, 0, 5] = top
+        rows[16 * i + 4, 0, 6] = -top
+    if dt == "f32":
+        rows[0, 0, 0] = 1e-45
+        rows[40] = 3e-39
+    k = rows.to(R.DT[dt]).cuda()
+    c = R.Case([(16, 16)] * 6, 1, dim, block, seed=1)
+    want = R.write_ref(c, k, -k)
+    e = enc()
+    kv8.encode_kv8_write(e, c.cache(), c.batch(), k, -k)
+    e.wait()
+    for s in range(6):
+        b = int(c.table_host[s, 0])
+        assert torch.equal(R.values(c.k)[b], want[0][b]) and torch.equal(R.values(c.v)[b], want[2][b])
+        assert float(c.ks[b]) == float(want[1][b]) and float(c.vs[b]) == float(want[3][b])
+    k[17, 0, 9] = float("nan")
+    want = R.write_ref(c, k, -k)
+    kv8.encode_kv8_write(e, c.cache(), c.batch(), k, -k)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 5
+    b = int(c.table_host[1, 0])
+    assert torch.equal(R.values(c.k)[b], want[0][b]) and not torch.isnan(R.values(c.v)[b]).any()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+LENS = [[(1, 1)], [(1, 15), (1, 16), (1, 17)], [(1, 63), (1, 64), (1, 65), (1, 1000)], [(4, 4), (2, 130), (0, 50), (3, 77)], [(1, 2500)]]
+
+
+def check_attn(c, q, out, was, scale, window, sinks):
+    ref, tol = R.attn_ref(c, q, was, scale, window, sinks)
+    end = c.start_host[-1]
+    assert torch.equal(out[end:], was[end:])                         # padding rows stay
+    d = (out.double() - ref).abs()
+    assert (d <= tol).all(), (float(d.max()), float((d / tol.clamp(min=1e-300))[:end].max()))
+
+
+@pytest.mark.parametrize("seqs", LENS)
+@pytest.mark.parametrize("kv_heads,G,dim,block", [(1, 1, 64, 16), (2, 8, 128, 64), (3, 5, 128, 16), (2, 7, 64, 128), (1, 40, 64, 32)])
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+def test_attention_of_few_rows(seqs, kv_heads, G, dim, block, dt):
+    from macseek_b200 import kv8
+    c = R.Case(seqs, kv_heads, dim, block, seed=dim + G, pad=2)
+    heads, scale = kv_heads * G, dim ** -0.5
+    e = enc()
+    cache, batch = c.cache(), c.batch()
+    scratch = kv8.attn_scratch(cache, batch, heads)
+    for window, sink, shift in ((0, False, 0), (0, True, 1), (20, False, 0), (1, True, 0), (700, False, 1)):
+        q, _ = spread(c.randn(c.rows, heads, dim, dt=dt, mul=3.0), 24, shift)
+        out, _ = spread(torch.full((c.rows, heads, dim), 7.0, dtype=R.DT[dt], device="cuda"), 8, shift)
+        was = out.clone()
+        sinks = c.randn(heads, mul=2.0) if sink else None
+        scratch.fill_(255)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, window=window, sinks=sinks)
+        e.wait()
+        check_attn(c, q, out, was, scale, window, sinks)
+
+
+@pytest.mark.parametrize("dt", ("f32", "bf16"))
+@pytest.mark.parametrize("dim", (64, 128))
+def test_attention_over_blocks_of_very_different_scales(dt, dim):
+    """Weights carry the blocks' value scales: neither a small one next to a large one nor the largest and smallest lose anything."""
+    from macseek_b200 import kv8
+    c = R.Case([(1, 200), (3, 120), (40, 200)], 1, dim, 16, seed=2)
+    for spread_v in (20, 35, 50):                                   # the widest that a cache has
+        c.vs.copy_(torch.exp2(torch.randint(-spread_v, spread_v + 1, c.vs.shape, generator=c.g).float()))
+        c.ks.copy_(torch.exp2(torch.randint(-14, -5, c.ks.shape, generator=c.g).float()))
+        cache, batch = c.cache(), c.batch()
+        q, out = c.randn(c.rows, 4, dim, dt=dt, mul=0.1), torch.zeros(c.rows, 4, dim, dtype=R.DT[dt], device="cuda")
+        e = enc()
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 4))
+        e.wait()
+        check_attn(c, q, out, out, dim ** -0.5, 0, None)
+
+
+def test_attention_results_do_not_depend_on_the_run_or_on_neighbours():
+    from macseek_b200 import kv8
+    c = R.Case([(1, 900), (1, 3000), (2, 64)], 2, 128, 64, seed=5)
+    q = c.randn(c.rows, 16, 128, dt="bf16")
+    cache, batch, e = c.cache(), c.batch(), enc()
+    outs = []
+    for _ in range(3):
+        out = torch.zeros_like(q)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 16))
+        outs.append(out)
+    e.wait()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_broken_batches_are_left_out_and_said():
+    """Numbers that cannot be right: that sequence is left out, the others are computed; a block that is not there is not seen."""
+    from macseek_b200 import _lib, kv8
+    e = enc()
+
+    def make():
+        return R.Case([(2, 40), (1, 33), (3, 50)], 2, 64, 16, seed=9)
+    for key, at, value in (("len", 1, -4), ("len", 1, 10 ** 6), ("len", 1, 0), ("start", 1, 100), ("start", 1, -2)):
+        c = make()
+        getattr(c, key)[at] = value
+        cache, batch = c.cache(), c.batch()
+        q = c.randn(c.rows, 4, 64)
+        out = torch.full_like(q, 7)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 4))
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 4
+        ref, tol = R.attn_ref(c, q, out, 0.125)
+        good = slice(3, 6) if key == "len" else slice(3, 6)
+        assert ((out.double() - ref).abs() <= tol)[good].all()
+        if key == "len":
+            assert (out[2] == 7).all()
+            assert ((out.double() - ref).abs() <= tol)[:2].all()
+        k = c.randn(c.rows, 2, 64)
+        kv8.encode_kv8_write(e, cache, batch, k, k)
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 4
+        kv8.encode_kv8_read(e, cache, batch, k, k.clone())
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 4
+    c = make()
+    full = c.table_host.clone()
+    c.table[2, 1] = -7                                                # tokens 16 .. 31 of the last sequence
+    cache, batch = c.cache(), c.batch()
+    q = c.randn(c.rows, 4, 64)
+    out = torch.zeros_like(q)
+    kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 4))
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 4
+    k, v = c.held(2, "k"), c.held(2, "v")
+    there = torch.tensor([p < 16 or p >= 32 for p in range(50)], device="cuda")
+    for i in range(3):
+        m = there & (torch.arange(50, device="cuda") <= 47 + i)
+        for h in range(4):
+            lg = (k[h // 2] @ q[3 + i, h].double() * 0.125).masked_fill(~m, -torch.inf)
+            assert ((torch.softmax(lg, 0) @ v[h // 2]) - out[3 + i, h].double()).abs().max() < 1e-4
+    c.table[2] = 999
+    out.fill_(7)
+    kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 4))
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 4
+    assert (out[3:] == 0).all()                                       # rows that see nothing
+    ko, vo = torch.full((c.rows, 2, 64), 7.0, device="cuda"), torch.full((c.rows, 2, 64), 7.0, device="cuda")
+    kv8.encode_kv8_read(e, cache, batch, ko, vo)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 4 and (ko[3:] == 0).all() and (vo[3:] == 0).all() and not (ko[:3] == 7).any()
+    was = c.k.clone()
+    kv8.encode_kv8_write(e, cache, c.batch(), ko, vo)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 4
+    kept = [int(i) for i in full[2, :4]]
+    assert torch.equal(c.k[kept], was[kept])
+
+
+def test_refusals_that_need_a_device():
+    from macseek_b200 import _lib, kv8
+    c = R.Case([(1, 5000)], 2, 128, 64, seed=1)
+    cache, batch = c.cache(), c.batch()
+    q = c.randn(c.rows, 16, 128)
+    e = enc()
+    small = torch.empty(64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(_lib.MsbError, match="scratch"):
+        kv8.encode_kv8_attn(e, cache, batch, q, torch.empty_like(q), small)
+    with pytest.raises(_lib.MsbError):
+        kv8.encode_kv8_attn(e, cache, batch, q, torch.empty_like(q).half(), kv8.attn_scratch(cache, batch, 16))
+    with pytest.raises(_lib.MsbError):
+        kv8.encode_kv8_attn(e, cache, batch, q.cpu(), torch.empty_like(q), kv8.attn_scratch(cache, batch, 16))
+    with pytest.raises(_lib.MsbError):
+        kv8.attn_scratch(cache, batch, 15)
+    e.wait()
