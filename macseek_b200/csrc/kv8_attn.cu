@@ -1,18 +1,19 @@
 // Attention over the 8-bit cache (kv8_attn.cuh) for few query rows: single tokens and short drafts.
 //
 // Every code is read once and what bounds the kernel is that read.  A block of four warps takes 16 rows of one key head (mma.sync
-// m16n8k16: a whole group of query heads, several tokens of a draft) over one range of keys; a warp takes every fourth step of 16 tokens.
-// Steps are fetched by the warp itself, with cp.async into its own ring, so that the warps never wait for one another before the end.
+// m16n8k16: a whole group of query heads, several tokens of a draft) over one range of keys; a warp takes every fourth step of 32 tokens.
+// Steps are fetched by the warp itself, with cp.async into its own two buffers, so that the warps never wait for one another before the end.
 //   scores   the contraction may run over the dims in any order: a lane takes 16 neighbouring bytes of "its" token as eight pairs and
 //            the query's registers are laid out alike; a pair of codes is one conversion to two halves (exact)
-//   output   the tokens are contracted: bytes of two neighbouring tokens are interleaved and converted; lane g holds dims [16 g, 16 g + 16)
+//   output   the tokens are contracted: bytes of two neighbouring tokens are interleaved and converted; lane g holds dims [g D / 8, (g + 1) D / 8)
+//   weights  the reference of the exponents moves only when a weight would pass 2^8: the sums are rescaled a few times, not at every new maximum
 // The queries are scaled by a power of two to at most 2 in a row and used as halves; F32 ones, and their weights, as two halves each.
 #include <algorithm>
 #include "kv8_attn.cuh"
 
 namespace msb {
 
-constexpr int kKdWarps = 4, kKdStages = 4, kKdStep = 16, kKdRows = 16;
+constexpr int kKdWarps = 4, kKdStages = 2, kKdStep = 32, kKdRows = 16, kKmStep = 128;
 
 __device__ __forceinline__ void kd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -43,7 +44,6 @@ __device__ __forceinline__ float kd_exp2(float x) {
 
 template <int D>
 struct KdTile {
-  static constexpr int kBytes = kKdStep * D;
   // where 16-byte chunk c of row r lies.  D 128: the keys' reads (rows r, r + 1; chunks t, t + 4) and the values' (rows 2 t, chunks g) are
   // free of bank conflicts with these; D 64: rows 4..7 and 12..15 change places in pairs as well
   static __device__ __forceinline__ uint32_t key(int r, int c) { return D == 128 ? r * 128 + ((c ^ ((r & 1) << 2)) << 4) : r * 64 + (c << 4); }
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   pdl_wait();
   constexpr bool TWO = sizeof(T) == 4;
   constexpr int KS = D / 16, NT = D / 8, CH = D / 64;      // k-steps, output tiles, 16-byte chunks of a key row per lane
-  constexpr int kWarpBytes = kKdStages * 2 * KdTile<D>::kBytes, kPitch = D + 4;
+  constexpr int kHalf = 16 * D, kStage = 4 * kHalf, kWarpBytes = kKdStages * kStage, kPitch = D + 4;     // keys of 32 tokens, their values
   extern __shared__ __align__(16) uint8_t kd_smem[];
   __shared__ float s_m[kKdWarps][kKdRows], s_l[kKdWarps][kKdRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -73,16 +73,15 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   const int steps = (k1 - k0 + kKdStep - 1) / kKdStep;
   const int mine = steps > warp ? (steps - warp + kKdWarps - 1) / kKdWarps : 0;
   const int* table = p.b.table + (size_t)blockIdx.z * p.b.table_stride;
-  const uint32_t ring = smem_u32(kd_smem) + warp * kWarpBytes;
 
-  // ---- block ids and scales of the warp's next 32 steps, one step per lane
+  // ---- block ids and scales of the warp's next 16 steps, half a step (16 tokens: one block) per lane; ve = -inf: no such block
   int ids = -1;
-  float ksc = 0.f, vex = 0.f;
+  float ksc = 0.f, vex = -INFINITY;
   auto look_up = [&](int i) {
-    const int step = warp + kKdWarps * (i + lane);
-    ids = -1; ksc = 0.f; vex = 0.f;
-    if (step < steps) {
-      ids = __ldg(table + ((k0 + kKdStep * step) >> p.c.shift));
+    const int key = k0 + kKdStep * (warp + kKdWarps * (i + (lane >> 1))) + 16 * (lane & 1);
+    ids = -1; ksc = 0.f; vex = -INFINITY;
+    if (key < k1) {
+      ids = __ldg(table + (key >> p.c.shift));
       if (ids < 0 || ids >= p.c.n_blocks) { ids = -1; atomicCAS(p.status, 0, kDevBadBatch); }
       else {
         ksc = __ldg(p.c.ks + (size_t)ids * p.c.heads + kvh);
@@ -90,27 +89,34 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
       }
     }
   };
+  // this lane's part of a copy: 16 bytes of rows r0, r0 + 512 / D, ...
+  const int r0 = lane / (D / 16), c0 = lane % (D / 16);
+  const uint32_t ring = smem_u32(kd_smem) + warp * kWarpBytes;
+  const uint32_t kd = ring + KdTile<D>::key(r0, c0);
+  const uint32_t vd[2] = {ring + 2 * kHalf + KdTile<D>::val(r0, c0), ring + 2 * kHalf + KdTile<D>::val(r0 + 512 / D, c0) - 512};
+  const uint8_t *ksrc = p.c.k + 16 * lane, *vsrc = p.c.v + 16 * lane;
   auto fetch = [&](int i) {                   // step i of the warp; its lane's ids are loaded
     if (i < mine) {
-      const int id = __shfl_sync(0xffffffffu, ids, i & 31);
       const int base = k0 + kKdStep * (warp + kKdWarps * i);
-      const size_t off = ((((size_t)max(id, 0) * p.c.heads + kvh) << p.c.shift) + (base & ((1 << p.c.shift) - 1))) * D;
-      const uint32_t dst = ring + (i % kKdStages) * 2 * KdTile<D>::kBytes;
+      const uint32_t st = (i & 1) * kStage;
 #pragma unroll
-      for (int j = 0; j < D / 32; j++) {
-        const int c = lane + 32 * j, r = c / (D / 16), ch = c % (D / 16);
-        const bool there = id >= 0 && base + r < sq.len;     // rows behind the last token hold anything
-        kd_copy16(dst + KdTile<D>::key(r, ch), p.c.k + off + c * 16, there);
-        kd_copy16(dst + KdTile<D>::kBytes + KdTile<D>::val(r, ch), p.c.v + off + c * 16, there);
+      for (int h = 0; h < 2; h++) {
+        const int id = __shfl_sync(0xffffffffu, ids, (2 * i + h) & 31), key = base + 16 * h;
+        const int rows = id >= 0 ? sq.len - key - r0 : 0;      // rows behind the last token hold anything: zeros for them
+        const size_t off = ((((size_t)max(id, 0) * p.c.heads + kvh) << p.c.shift) + (key & ((1 << p.c.shift) - 1))) * D;
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+          const bool there = rows > j * (512 / D);
+          kd_copy16(kd + st + h * kHalf + 512 * j, ksrc + off + 512 * j, there);
+          kd_copy16(vd[j & 1] + st + h * kHalf + 512 * j, vsrc + off + 512 * j, there);
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   look_up(0);
   float ks_cur = ksc, ve_cur = vex;           // of the batch that is being computed (the fetches run ahead into the next one)
-  int id_cur = ids;
-#pragma unroll
-  for (int i = 0; i < kKdStages - 1; i++) fetch(i);
+  fetch(0);
 
   // ---- queries: rows g and g + 8 of the tile, scaled to at most 2
   uint32_t qh[KS][4], ql[TWO ? KS : 1][4];
@@ -120,7 +126,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   for (int h = 0; h < 2; h++) {
     const int r = m0 + g + 8 * h, tok = min(r, R - 1) / p.G, head = kvh * p.G + min(r, R - 1) % p.G;
     const T* src = static_cast<const T*>(p.q) + (sq.row + tok) * p.q_stride + (int64_t)head * D;
-    qpos[h] = r < R ? sq.len - sq.n + tok : -1;              // a row that is not there sees nothing
+    qpos[h] = sq.len - sq.n + tok;
     float v[CH][16];
     float top = 0.f;
 #pragma unroll
@@ -148,113 +154,132 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
         if (TWO) { ql[4 * j + i][h] = lo[0]; ql[4 * j + i][2 + h] = lo[1]; }
       }
   }
+  // keys that every row of the tile sees: no comparisons for steps inside them
+  const int all_hi = min(k1, sq.len - sq.n + m0 / p.G + 1), all_lo = p.window ? sq.len - sq.n + (m1 - 1) / p.G - p.window + 1 : 0;
 
   float o[NT][4];
 #pragma unroll
   for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const uint8_t* kbase = kd_smem + warp * kWarpBytes;
+  const uint8_t* own = kd_smem + warp * kWarpBytes;
+  const uint8_t* kl = own + KdTile<D>::key(g, t);
+  const uint8_t* vl[2] = {own + 2 * kHalf + KdTile<D>::val(2 * t, D == 128 ? g : g >> 1) + (D == 128 ? 0 : 8 * (g & 1)),
+                          own + 2 * kHalf + KdTile<D>::val(2 * t + 1, D == 128 ? g : g >> 1) + (D == 128 ? 0 : 8 * (g & 1))};
+  const int flip = (g & 1) ? -64 : 64;        // a key row's other chunk (D 128)
 
   for (int i = 0; i < mine; i++) {
-    if (i + kKdStages - 1 < mine && ((i + kKdStages - 1) & 31) == 0) look_up(i + kKdStages - 1);
-    fetch(i + kKdStages - 1);
-    if (i && (i & 31) == 0) { ks_cur = ksc; ve_cur = vex; id_cur = ids; }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kKdStages - 1) : "memory");
+    if (i + 1 < mine && ((i + 1) & 15) == 0) look_up(i + 1);
+    fetch(i + 1);
+    if (i && (i & 15) == 0) { ks_cur = ksc; ve_cur = vex; }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
-    const uint8_t* kt = kbase + (i % kKdStages) * 2 * KdTile<D>::kBytes;
-    const uint8_t* vt = kt + KdTile<D>::kBytes;
+    const uint32_t st = (i & 1) * kStage;
     const int base = k0 + kKdStep * (warp + kKdWarps * i);
-    const float ks = __shfl_sync(0xffffffffu, ks_cur, i & 31), ve = __shfl_sync(0xffffffffu, ve_cur, i & 31);
-    const bool ok = __shfl_sync(0xffffffffu, id_cur, i & 31) >= 0;
-    // ---- scores of 16 tokens
-    float s[2][4];
+    float ks[2], ve[2];
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
-      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int h = 0; h < 2; h++) {
+      ks[h] = __shfl_sync(0xffffffffu, ks_cur, (2 * i + h) & 31);
+      ve[h] = __shfl_sync(0xffffffffu, ve_cur, (2 * i + h) & 31);
+    }
+    // ---- scores of 32 tokens
+    float s[4][4];
 #pragma unroll
-      for (int j = 0; j < CH; j++) {
-        const uint4 u = *reinterpret_cast<const uint4*>(kt + KdTile<D>::key(8 * nt + g, t + 4 * j));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int nt = 0; nt < 4; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-          const uint32_t b0 = kv8_half2(w[x]), b1 = kv8_half2(w[x] >> 16);
+    for (int j = 0; j < CH; j++) {
+      uint32_t w[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 4; nt++) {
+        const uint4 u = *reinterpret_cast<const uint4*>(kl + st + nt * 8 * D + (j ? flip : 0));
+        w[nt][0] = u.x; w[nt][1] = u.y; w[nt][2] = u.z; w[nt][3] = u.w;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+#pragma unroll
+        for (int nt = 0; nt < 4; nt++) {
+          const uint32_t b0 = kv8_half2(w[nt][x]), b1 = kv8_half2(w[nt][x] >> 16);
           kd_mma(s[nt], qh[4 * j + x], b0, b1);
           if (TWO) kd_mma(s[nt], ql[4 * j + x], b0, b1);
         }
-      }
     }
-    // ---- weights
-    float top[2] = {-INFINITY, -INFINITY};
+    // ---- weights: rows (r >> 1), tokens 8 nt + 2 t + (r & 1)
+#pragma unroll
+    for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[nt][r] = fmaf(s[nt][r], qs[r >> 1] * ks[nt >> 1], ve[nt >> 1]);
+    if (base + kKdStep > all_hi || base < all_lo) {
+#pragma unroll
+      for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int key = base + 8 * nt + 2 * t + (r & 1), pos = qpos[r >> 1];
+          if (key >= k1 || key > pos || (p.window && key <= pos - p.window)) s[nt][r] = -INFINITY;
+        }
+    }
+    float top[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const float f = qs[h] * ks;
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int key = base + 8 * nt + 2 * t + x;
-          const bool seen = ok && key < k1 && key <= qpos[h] && (!p.window || key > qpos[h] - p.window);
-          float& v = s[nt][2 * h + x];
-          v = seen ? fmaf(v, f, ve) : -INFINITY;
-          top[h] = fmaxf(top[h], v);
-        }
+      top[h] = fmaxf(fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])),
+                     fmaxf(fmaxf(s[2][2 * h], s[2][2 * h + 1]), fmaxf(s[3][2 * h], s[3][2 * h + 1])));
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float n = fmaxf(m[h], top[h]), f = n == -INFINITY ? 1.f : kd_exp2(m[h] - n);
+        const float n = top[h] > m[h] + 8.f ? top[h] : m[h], f = n == -INFINITY ? 1.f : kd_exp2(m[h] - n);
         m[h] = n; l[h] *= f;
 #pragma unroll
         for (int k = 0; k < NT; k++) { o[k][2 * h] *= f; o[k][2 * h + 1] *= f; }
       }
     }
-    const float vi = kv8_pow2(-(int)ve);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const float mm = m[h] == -INFINITY ? 0.f : m[h];
-      float sum = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++)
+      for (int x = 0; x < 2; x++) {           // halves of the step: a block and its value scale each
+        float sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          float& v = s[nt][2 * h + x];
+        for (int y = 0; y < 4; y++) {
+          float& v = s[2 * x + (y >> 1)][2 * h + (y & 1)];
           v = kd_exp2(v - mm);
           sum += v;
         }
-      l[h] = fmaf(sum, vi, l[h]);
-    }
-    uint32_t ph[4], pl[4];
-    kd_split<TWO>(s[0][0], s[0][1], ph[0], pl[0]);
-    kd_split<TWO>(s[0][2], s[0][3], ph[1], pl[1]);
-    kd_split<TWO>(s[1][0], s[1][1], ph[2], pl[2]);
-    kd_split<TWO>(s[1][2], s[1][3], ph[3], pl[3]);
-    // ---- output: lane g has dims [g D / 8, (g + 1) D / 8), tile j its j-th
-    uint32_t x[4][NT / 4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int row = 2 * t + (r & 1) + 8 * (r >> 1);
-      if (D == 128) {
-        const uint4 u = *reinterpret_cast<const uint4*>(vt + KdTile<D>::val(row, g));
-        x[r][0] = u.x; x[r][1] = u.y; x[r][NT / 4 - 2] = u.z; x[r][NT / 4 - 1] = u.w;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(vt + KdTile<D>::val(row, g >> 1) + 8 * (g & 1));
-        x[r][0] = u.x; x[r][1] = u.y;
+        l[h] = fmaf(sum, ve[x] == -INFINITY ? 0.f : kv8_pow2(-(int)ve[x]), l[h]);
       }
     }
+    // ---- output
 #pragma unroll
-    for (int w = 0; w < NT / 4; w++) {
-      const uint32_t a0 = __byte_perm(x[0][w], x[1][w], 0x5140), a1 = __byte_perm(x[0][w], x[1][w], 0x7362);
-      const uint32_t c0 = __byte_perm(x[2][w], x[3][w], 0x5140), c1 = __byte_perm(x[2][w], x[3][w], 0x7362);
+    for (int h = 0; h < 2; h++) {
+      uint32_t ph[4], pl[4], x[4][NT / 4];
+      kd_split<TWO>(s[2 * h][0], s[2 * h][1], ph[0], pl[0]);
+      kd_split<TWO>(s[2 * h][2], s[2 * h][3], ph[1], pl[1]);
+      kd_split<TWO>(s[2 * h + 1][0], s[2 * h + 1][1], ph[2], pl[2]);
+      kd_split<TWO>(s[2 * h + 1][2], s[2 * h + 1][3], ph[3], pl[3]);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const uint32_t b0 = kv8_half2((e < 2 ? a0 : a1) >> (16 * (e & 1))), b1 = kv8_half2((e < 2 ? c0 : c1) >> (16 * (e & 1)));
-        kd_mma(o[4 * w + e], ph, b0, b1);
-        if (TWO) kd_mma(o[4 * w + e], pl, b0, b1);
+      for (int r = 0; r < 4; r++) {           // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        const uint8_t* src = vl[r & 1] + st + h * kHalf + (r >> 1) * 8 * D;
+        if (D == 128) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src);
+          x[r][0] = u.x; x[r][1] = u.y; x[r][NT / 4 - 2] = u.z; x[r][NT / 4 - 1] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          x[r][0] = u.x; x[r][1] = u.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < NT / 4; w++) {
+        const uint32_t a0 = __byte_perm(x[0][w], x[1][w], 0x5140), a1 = __byte_perm(x[0][w], x[1][w], 0x7362);
+        const uint32_t c0 = __byte_perm(x[2][w], x[3][w], 0x5140), c1 = __byte_perm(x[2][w], x[3][w], 0x7362);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t b0 = kv8_half2((e < 2 ? a0 : a1) >> (16 * (e & 1))), b1 = kv8_half2((e < 2 ? c0 : c1) >> (16 * (e & 1)));
+          kd_mma(o[4 * w + e], ph, b0, b1);
+          if (TWO) kd_mma(o[4 * w + e], pl, b0, b1);
+        }
       }
     }
-    __syncwarp();                              // every lane has read the stage that the next fetch fills
+    __syncwarp();                              // every lane has read the buffer that the next fetch fills
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -328,7 +353,7 @@ __global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnParams 
   const int i = tok - sq.row;
   if (i < 0 || i >= sq.n) return;
   const int row = i * p.G + head % p.G, m0 = row / p.tile * p.tile, m1 = min(m0 + p.tile, sq.n * p.G);
-  const Kv8Range kr = kv8_range(sq, m0, m1, p.G, p.window, kKdStep);
+  const Kv8Range kr = kv8_range(sq, m0, m1, p.G, p.window, p.step);
   const int n = (kr.hi - kr.lo + p.chunk - 1) / p.chunk;
   const size_t stride = (size_t)p.b.n_tokens * p.heads, at = (size_t)tok * p.heads + head;
   const float2* ml = reinterpret_cast<const float2*>(kv8_part_ml(p, D)) + at;
@@ -374,17 +399,20 @@ __global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnParams 
 }
 
 // ---------------------------------------------------------------- host side
-struct Kv8Plan { int tiles, chunk, splits, most; };      // most: splits at most, for any window
-static Kv8Plan kv8_plan(const Kv8Batch& b, int kv_heads, int heads, int window, int sms) {
+struct Kv8Plan { int many, tiles, chunk, splits, most; };      // most: splits at most, for any window
+static Kv8Plan kv8_plan(const Kv8Batch& b, int kv_heads, int heads, int window, int elem_type, int sms) {
   const int G = heads / kv_heads;
   Kv8Plan pl;
-  pl.tiles = (int)(((int64_t)b.max_new * G + kKdRows - 1) / kKdRows);
+  pl.many = (int64_t)b.max_new * G > 32;
+  const int rows = pl.many ? kv8_many_rows(elem_type) : kKdRows, step = pl.many ? kKmStep : kKdStep;
+  pl.tiles = (int)(((int64_t)b.max_new * G + rows - 1) / rows);
   const int64_t units = (int64_t)pl.tiles * kv_heads * b.n_seq;
-  // three blocks an SM; several sequences, whose lengths differ, in three waves
-  const int64_t want = (int64_t)3 * sms * (b.n_seq > 1 ? 3 : 1);
-  const Kv8Split sp = kv8_split(kv8_span(b.max_len, kKdRows, G, window, kKdStep), units, want, 128);
+  // few rows: three blocks an SM, and six times as many for sequences whose lengths differ
+  const int64_t want = pl.many ? 2 * sms : (int64_t)3 * sms * (b.n_seq > 1 ? 6 : 1);
+  const int least = pl.many ? 512 : 128;
+  const Kv8Split sp = kv8_split(kv8_span(b.max_len, rows, G, window, step), units, want, least, pl.many ? kKmStep : 64);
   pl.chunk = sp.chunk; pl.splits = sp.splits;
-  pl.most = kv8_most_splits(b.max_len, units, want, 128);
+  pl.most = kv8_most_splits(b.max_len, units, want, least);
   return pl;
 }
 static int kv8_sms(int* sms) {
@@ -400,24 +428,30 @@ static int kv8_heads_check(const msb_kv8_cache* c, int heads, const char* what) 
 static size_t kv8_part_bytes(const Kv8Batch& b, int heads, int D, int splits) {
   return splits > 1 ? sizeof(float) * (size_t)splits * b.n_tokens * heads * (D + 2) : 0;
 }
-size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, int heads) {
+size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, int heads) {      // for rows of any type
   Kv8Cache cc; Kv8Batch bb;
   int sms;
   if (kv8_check(c, b, "kv8_attn_scratch_bytes", &cc, &bb) || kv8_heads_check(c, heads, "kv8_attn_scratch_bytes") || kv8_sms(&sms)) return 0;
-  return 16 + kv8_part_bytes(bb, heads, c->head_dim, kv8_plan(bb, cc.heads, heads, 0, sms).most);
+  const int most = std::max(kv8_plan(bb, cc.heads, heads, 0, F32, sms).most, kv8_plan(bb, cc.heads, heads, 0, BF16, sms).most);
+  return 16 + kv8_part_bytes(bb, heads, c->head_dim, most);
 }
 
 template <class T, int D>
-static int launch_attn(Kv8AttnParams& p, const Kv8Plan& pl, cudaStream_t st, int dev) {
-  auto kern = kv8_attn_few_kernel<T, D>;
-  const size_t smem = std::max<size_t>((size_t)kKdWarps * kKdStages * 2 * KdTile<D>::kBytes, sizeof(float) * kKdWarps * kKdRows * (D + 4));
-  static bool done[64] = {};
-  if (!done[dev & 63]) {
-    MSB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    done[dev & 63] = true;
+static int launch_attn(const Kv8AttnParams& p, const Kv8Plan& pl, int elem_type, cudaStream_t st, int dev) {
+  if (pl.many) {
+    const int rc = kv8_attn_many(p, pl.tiles, elem_type, D, st, dev);
+    if (rc) return rc;
+  } else {
+    auto kern = kv8_attn_few_kernel<T, D>;
+    const size_t smem = std::max<size_t>((size_t)kKdWarps * kKdStages * 2 * kKdStep * D, sizeof(float) * kKdWarps * kKdRows * (D + 4));
+    static bool done[64] = {};
+    if (!done[dev & 63]) {
+      MSB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      done[dev & 63] = true;
+    }
+    MSB_CUDA(launch_pdl(kern, dim3(pl.splits, p.c.heads * pl.tiles, p.b.n_seq), dim3(kKdWarps * 32), smem, st, p));
+    MSB_LAUNCH_CHECK("kv8_attn");
   }
-  MSB_CUDA(launch_pdl(kern, dim3(pl.splits, p.c.heads * pl.tiles, p.b.n_seq), dim3(kKdWarps * 32), smem, st, p));
-  MSB_LAUNCH_CHECK("kv8_attn");
   if (pl.splits > 1) {
     MSB_CUDA(launch_pdl(kv8_attn_join_kernel<T, D>, dim3(p.b.n_tokens, p.heads), dim3(128), 0, st, p));
     MSB_LAUNCH_CHECK("kv8_attn_join");
@@ -439,17 +473,18 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   int dev, sms;
   MSB_CUDA(cudaGetDevice(&dev));
   if ((rc = kv8_sms(&sms))) return rc;
-  const Kv8Plan pl = kv8_plan(p.b, p.c.heads, heads, window, sms);
-  if ((int64_t)p.c.heads * pl.tiles > 65535) return fail(kErrLimit, "%s: too many rows", what);
+  const Kv8Plan pl = kv8_plan(p.b, p.c.heads, heads, window, elem_type, sms);
+  if (pl.many ? pl.tiles > 65535 : (int64_t)p.c.heads * pl.tiles > 65535) return fail(kErrLimit, "%s: too many rows", what);
   const size_t need = kv8_part_bytes(p.b, heads, c->head_dim, pl.splits);
   if (need && (!scratch || scratch_bytes < need)) return fail(kErrScratch, "%s: scratch too small (%zu < %zu)", what, scratch_bytes, need);
   if (need && (reinterpret_cast<uintptr_t>(scratch) & 15)) return fail(kErrArg, "%s: scratch must be 16-byte aligned", what);
   Tables tb;
   if ((rc = get_tables(&tb))) return rc;
   p.q = q; p.out = out; p.q_stride = q_stride; p.out_stride = out_stride; p.sinks = sinks; p.part = static_cast<float*>(scratch);
-  p.scale = scale; p.heads = heads; p.G = heads / p.c.heads; p.window = window; p.chunk = pl.chunk; p.splits = pl.splits; p.tile = kKdRows;
+  p.scale = scale; p.heads = heads; p.G = heads / p.c.heads; p.window = window; p.chunk = pl.chunk; p.splits = pl.splits;
+  p.tile = pl.many ? kv8_many_rows(elem_type) : kKdRows; p.step = pl.many ? kKmStep : kKdStep;
   p.q_vec = qv; p.out_vec = ov; p.status = tb.status;
-#define KV8_GO(T) return c->head_dim == 64 ? launch_attn<T, 64>(p, pl, st, dev) : launch_attn<T, 128>(p, pl, st, dev)
+#define KV8_GO(T) return c->head_dim == 64 ? launch_attn<T, 64>(p, pl, elem_type, st, dev) : launch_attn<T, 128>(p, pl, elem_type, st, dev)
   if (elem_type == F32) KV8_GO(float);
   if (elem_type == F16) KV8_GO(__half);
   KV8_GO(__nv_bfloat16);

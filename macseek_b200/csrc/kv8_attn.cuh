@@ -20,10 +20,14 @@ struct Kv8AttnParams {
   const float* sinks;
   float* part;                 // [splits][n_tokens * heads][D], then [splits][n_tokens * heads] of (m, sum)
   float scale;
-  int heads, G, window, chunk, splits, tile;   // keys of one split (a multiple of the kernel's step), splits at most, rows of a tile
+  int heads, G, window;
+  int chunk, splits, tile, step;   // keys of one split (a multiple of step), splits at most, rows of a tile, keys of a step
   int q_vec, out_vec;
   int* status;
 };
+
+int kv8_many_rows(int elem_type);      // rows of a block of the kernel for many rows, and its launch over `groups` blocks of rows
+int kv8_attn_many(const Kv8AttnParams& p, int groups, int elem_type, int D, cudaStream_t st, int dev);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ float* kv8_part_ml(const Kv8AttnParams& p, int D) {

@@ -67,11 +67,11 @@ inline int kv8_span(int max_len, int rows, int G, int window, int step) {
   return window && w < max_len ? (int)w : max_len;
 }
 
-// Split of the keys: `units` blocks of threads without one, about `want` blocks wanted; chunks of at least `least` keys, a multiple of 64.
+// Split of the keys: `units` blocks of threads without one, about `want` blocks wanted; chunks of at least `least` keys, a multiple of `step`.
 struct Kv8Split { int chunk, splits; };
-inline Kv8Split kv8_split(int span, int64_t units, int64_t want, int least) {
+inline Kv8Split kv8_split(int span, int64_t units, int64_t want, int least, int step = 64) {
   const int64_t n = want / (units > 0 ? units : 1) > 1 ? want / units : 1;
-  int64_t chunk = ((span + n - 1) / n + 63) / 64 * 64;
+  int64_t chunk = ((span + n - 1) / n + step - 1) / step * step;
   if (chunk < least) chunk = least;
   return Kv8Split{(int)chunk, (int)((span + chunk - 1) / chunk)};
 }

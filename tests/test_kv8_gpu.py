@@ -236,6 +236,32 @@ def test_attention_of_few_rows(seqs, kv_heads, G, dim, block, dt):
         check_attn(c, q, out, was, scale, window, sinks)
 
 
+CHUNKS = [[(128, 128)], [(129, 129), (127, 300)], [(33, 33), (1, 500), (0, 20), (300, 700)], [(64, 5000)], [(1000, 1000)], [(17, 2049), (65, 65)]]
+
+
+@pytest.mark.parametrize("seqs", CHUNKS)
+@pytest.mark.parametrize("kv_heads,G,dim,block", [(2, 8, 128, 64), (1, 1, 64, 16), (3, 5, 128, 16), (2, 7, 64, 128), (1, 16, 64, 32), (1, 130, 128, 64)])
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+def test_attention_of_many_rows(seqs, kv_heads, G, dim, block, dt):
+    from macseek_b200 import kv8
+    if G == 130:
+        seqs = [(min(n, 3), l) for n, l in seqs]                     # one token is more than a tile of rows
+    c = R.Case(seqs, kv_heads, dim, block, seed=dim + G, pad=2)
+    heads, scale = kv_heads * G, dim ** -0.5
+    e = enc()
+    cache, batch = c.cache(), c.batch()
+    scratch = kv8.attn_scratch(cache, batch, heads)
+    for window, sink, shift, sc in ((0, False, 0, scale), (0, True, 1, scale), (50, False, 0, -scale), (1, True, 0, 2 * scale), (300, False, 1, scale)):
+        q, _ = spread(c.randn(c.rows, heads, dim, dt=dt, mul=3.0), 24, shift)
+        out, _ = spread(torch.full((c.rows, heads, dim), 7.0, dtype=R.DT[dt], device="cuda"), 8, shift)
+        was = out.clone()
+        sinks = c.randn(heads, mul=2.0) if sink else None
+        scratch.fill_(255)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, scale=sc, window=window, sinks=sinks)
+        e.wait()
+        check_attn(c, q, out, was, sc, window, sinks)
+
+
 @pytest.mark.parametrize("dt", ("f32", "bf16"))
 @pytest.mark.parametrize("dim", (64, 128))
 def test_attention_over_blocks_of_very_different_scales(dt, dim):
