@@ -80,13 +80,19 @@ __device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float 
   return r;
 }
 
-// eight elements of a row; vec: 16-byte aligned
+// eight elements of a row; vec: 16-byte aligned (raw: always)
 template <class T> struct Elems;
 template <> struct Elems<float> {
+  struct Raw { uint4 a, b; };                                         // eight elements as they lie in memory
+  static __device__ __forceinline__ Raw raw(const float* p) { return Raw{reinterpret_cast<const uint4*>(p)[0], reinterpret_cast<const uint4*>(p)[1]}; }
+  static __device__ __forceinline__ void open(const Raw& r, float (&v)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(w[i]);
+  }
   static __device__ __forceinline__ void load(const float* p, bool vec, float (&v)[8]) {
     if (vec) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      open(raw(p), v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = p[i];
@@ -104,15 +110,19 @@ template <> struct Elems<float> {
   static __device__ __forceinline__ float from(float x) { return x; }
 };
 template <class T, class T2> struct Elems16 {
+  typedef uint4 Raw;
+  static __device__ __forceinline__ Raw raw(const T* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ void open(const Raw& u, float (&v)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const T2 h = *reinterpret_cast<const T2*>(&w[i]);
+      v[2 * i] = static_cast<float>(h.x); v[2 * i + 1] = static_cast<float>(h.y);
+    }
+  }
   static __device__ __forceinline__ void load(const T* p, bool vec, float (&v)[8]) {
     if (vec) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const T2 h = *reinterpret_cast<const T2*>(&w[i]);
-        v[2 * i] = static_cast<float>(h.x); v[2 * i + 1] = static_cast<float>(h.y);
-      }
+      open(raw(p), v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = static_cast<float>(p[i]);

@@ -22,18 +22,19 @@ template <class T, int D>
 struct KmShape {
   static constexpr bool kTwo = sizeof(T) == 4;
   static constexpr int kTiles = kTwo ? 1 : 2, kTerms = kTwo ? 2 : 1;
-  static constexpr int kSoft = 4 * kTiles, kWarps = kSoft + 5;
+  static constexpr int kSoft = 4 * kTiles, kMma = kSoft + 4, kWarps = kMma + 1;
   static constexpr int kBytes = 128 * D * 2;                          // a tile of 128 rows as halves
-  static constexpr int kSmem = 2048 + kTiles * kTerms * kBytes + 4 * kBytes;
+  static constexpr int kSmem = 3072 + kTiles * kTerms * kBytes + 4 * kBytes;
   static constexpr uint32_t kO = 256, kLow = 128;
 };
 struct KmHead {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], ofull[2], qfull;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2][2], ahalf[2], ofull[2], qfull;      // pfull: of a tile's first and second 64 keys
   uint32_t tmem_base;
   int abort_flag;
+  float f0[2 * kKmRows];
   float4 sc[2][kKmKeys / 16];       // key scale, exponent of the value scale, its inverse; of 16 tokens of a tile
 };
-static_assert(sizeof(KmHead) <= 1024, "the tiles follow");
+static_assert(sizeof(KmHead) <= 2048, "the tiles follow");
 
 // place of the 16 bytes `j` of row r, 64 halves a row: 8-row groups of 1024 bytes, 128-byte swizzle
 __device__ __forceinline__ uint32_t km_at(int r, int j) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((j ^ (r & 7)) << 4)); }
@@ -59,6 +60,41 @@ __device__ __forceinline__ float km_exp2(float x) {
   return y;
 }
 
+// two f32 at a time
+__device__ __forceinline__ uint64_t km_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void km_apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t km_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t km_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// 2^x of two numbers on the fused multiply-add pipe: x = n + r, |r| <= 1/2, a polynomial of degree 4 in r (minimax by Remez exchange, 2^-18.5)
+// and n into its exponent.  [-126, 127]; what is below is as good as 0, what is above is looked at again
+__device__ __forceinline__ void km_exp2_fma(float& a, float& b) {
+  const float big = 12582912.f;                        // 1.5 * 2^23: the sum's last bits are the nearest whole number
+  const uint64_t x = km_two(fminf(fmaxf(a, -126.f), 127.f), fminf(fmaxf(b, -126.f), 127.f));
+  const uint64_t t = km_add2(x, km_two(big, big)), r = km_fma2(km_add2(t, km_two(-big, -big)), km_two(-1.f, -1.f), x);
+  uint64_t p = km_fma2(r, km_two(0.009570102207362652f, 0.009570102207362652f), km_two(0.05591785907745361f, 0.05591785907745361f));
+  p = km_fma2(p, r, km_two(0.240247443318367f, 0.240247443318367f));
+  p = km_fma2(p, r, km_two(0.6931217908859253f, 0.6931217908859253f));
+  p = km_fma2(p, r, km_two(0.9999992847442627f, 0.9999992847442627f));
+  float pa, pb, ta, tb;
+  km_apart(p, pa, pb);
+  km_apart(t, ta, tb);
+  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
+}
+
 template <class T, int D>
 __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_kernel(const Kv8AttnParams p) {
   using S = KmShape<T, D>;
@@ -66,7 +102,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
   extern __shared__ __align__(1024) uint8_t km_smem_raw[];
   uint8_t* smem = km_smem_raw + ((1024u - (smem_u32(km_smem_raw) & 1023u)) & 1023u);
   KmHead* hd = reinterpret_cast<KmHead*>(smem);
-  uint8_t* qs_mem = smem + 1024;                                       // [tiles][terms][kBytes]
+  uint8_t* qs_mem = smem + 2048;                                       // [tiles][terms][kBytes]
   uint8_t* kmem = qs_mem + S::kTiles * S::kTerms * S::kBytes;          // [2][kBytes]
   uint8_t* vmem = kmem + 2 * S::kBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -85,13 +121,13 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
   if (tid == 0) {
     for (int s = 0; s < 2; s++) {
       mbar_init(&hd->kfull[s], 4); mbar_init(&hd->kempty[s], 1); mbar_init(&hd->vfull[s], 4); mbar_init(&hd->vempty[s], 1);
-      mbar_init(&hd->sfull[s], 1); mbar_init(&hd->pfull[s], 4); mbar_init(&hd->ofull[s], 1);
+      mbar_init(&hd->sfull[s], 1); mbar_init(&hd->pfull[s][0], 4); mbar_init(&hd->pfull[s][1], 4); mbar_init(&hd->ahalf[s], 1); mbar_init(&hd->ofull[s], 1);
     }
     mbar_init(&hd->qfull, 4 * nt);
     hd->abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == S::kWarps - 1) {
+  if (warp == S::kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hd->tmem_base)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -104,249 +140,352 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, abort_flag, p.status, code)) != 0;
   };
 
-  if (warp == S::kWarps - 1) {
+  if (warp == S::kMma) {
     // ------------------------------------------------------------------ products
     constexpr uint32_t base = (1u << 4) | ((uint32_t)(kKmRows >> 4) << 24);
     constexpr uint32_t is = base | ((uint32_t)(kKmKeys >> 3) << 17), io = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     const bool leader = elect_one();
-    const uint32_t q_s = smem_u32(qs_mem), k_s = smem_u32(kmem), v_s = smem_u32(vmem);
-    auto scores = [&](int t, int s) {
-#pragma unroll
-      for (int e = 0; e < S::kTerms; e++)
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t o = (k >> 2) * 16384 + (k & 3) * 32;
-          km_mma_ss(tmem + t * 128, ts_desc(q_s + (t * S::kTerms + e) * S::kBytes + o), ts_desc(k_s + s * S::kBytes + o), is, (e | k) ? 1u : 0u);
-        }
-      ts_commit(&hd->sfull[t]);
-    };
-    bool ok = wait(&hd->qfull, 0, kDevWaitFull) && wait(&hd->kfull[0], 0, kDevWaitFull);
-    if (ok) {
-      ts_fence_after();
-      if (leader) {
-        for (int t = 0; t < nt; t++) scores(t, 0);
-        ts_commit(&hd->kempty[0]);
-      }
-      __syncwarp();
-    }
-    for (int j = 0; ok && j < n; j++) {
+    const uint64_t q_d = ts_desc(smem_u32(qs_mem)), k_d = ts_desc(smem_u32(kmem)), v_d = km_desc_mn(smem_u32(vmem), 16384);
+    bool ok = wait(&hd->qfull, 0, kDevWaitFull);
+    // round j: the output's products of tile j, then the scores of tile j + 1 (one copy of the code: it has to stay in the instruction cache)
+#pragma unroll 1
+    for (int j = -1; ok && j < n; j++) {
       const int s = j & 1;
-      ok = wait(&hd->vfull[s], j >> 1, kDevWaitFull);
+      const bool more = j + 1 < n;
+      ok = j < 0 || wait(&hd->vfull[s], j >> 1, kDevWaitFull);
+#pragma unroll 1
       for (int t = 0; ok && t < nt; t++) {
-        ok = wait(&hd->pfull[t], j, kDevWaitFull) && (t || j + 1 >= n || wait(&hd->kfull[s ^ 1], (j + 1) >> 1, kDevWaitFull));
+#pragma unroll 1
+        for (int h = 0; j >= 0 && h < 2; h++) {
+          ok = wait(&hd->pfull[t][h], j, kDevWaitFull);
+          if (!ok) break;
+          ts_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int e = 0; e < S::kTerms; e++)
+#pragma unroll
+              for (int k = 0; k < kKmKeys / 32; k++)
+                ts_mma_f16(tmem + S::kO + t * D, tmem + (e ? S::kLow : t * 128) + h * 32 + k * 8,
+                           v_d + (uint32_t)(s * (S::kBytes >> 4) + h * 512 + k * 128), io, (j | h | e | k) ? 1u : 0u);
+            if (h == 0) ts_commit(&hd->ahalf[t]);
+          }
+          __syncwarp();
+        }
+        ok = ok && (t || !more || wait(&hd->kfull[s ^ 1], (j + 1) >> 1, kDevWaitFull));
         if (!ok) break;
         ts_fence_after();
         if (leader) {
+          if (more) {
 #pragma unroll
-          for (int e = 0; e < S::kTerms; e++)
+            for (int e = 0; e < S::kTerms; e++)
 #pragma unroll
-            for (int k = 0; k < kKmKeys / 16; k++)
-              ts_mma_f16(tmem + S::kO + t * D, tmem + (e ? S::kLow : t * 128) + k * 8, km_desc_mn(v_s + s * S::kBytes + k * 2048, 16384), io,
-                         (j | e | k) ? 1u : 0u);
-          if (j + 1 < n) scores(t, s ^ 1);
-          else ts_commit(&hd->ofull[t]);
+              for (int k = 0; k < D / 16; k++) {
+                constexpr uint32_t step[2] = {16384 >> 4, 32 >> 4};
+                const uint32_t o = (k >> 2) * step[0] + (k & 3) * step[1];
+                km_mma_ss(tmem + t * 128, q_d + ((t * S::kTerms + e) * (S::kBytes >> 4) + o), k_d + ((s ^ 1) * (S::kBytes >> 4) + o), is, (e | k) ? 1u : 0u);
+              }
+            ts_commit(&hd->sfull[t]);
+          } else {
+            ts_commit(&hd->ofull[t]);
+          }
         }
         __syncwarp();
       }
       if (ok && leader) {
-        ts_commit(&hd->vempty[s]);
-        if (j + 1 < n) ts_commit(&hd->kempty[s ^ 1]);
+        if (j >= 0) ts_commit(&hd->vempty[s]);
+        if (more) ts_commit(&hd->kempty[s ^ 1]);
       }
       __syncwarp();
     }
-  } else if (warp >= S::kSoft) {
+  } else if (warp >= S::kSoft && warp < S::kMma) {
     // ------------------------------------------------------------------ codes -> halves
-    constexpr int kPer = D / 16;                       // 16-byte pieces a thread has of a tile
-    const int c = tid - S::kSoft * 32, pc = c % (D / 16), row0 = c / (D / 16);
+    constexpr int kPer = D / 16, kRows = 128 / kPer;   // 16-byte pieces a thread has of a tile, kRows rows apart
+    // a quarter of a warp has two rows' pieces of one 64-dim half: its stores meet no bank twice
+    const int c = tid - S::kSoft * 32, pc = D == 128 ? (c & 3) | (c >> 1 & 4) : c & 3, row0 = D == 128 ? (c >> 2 & 1) | (c >> 4) << 1 : c >> 2;
     const int* table = p.b.table + (size_t)blockIdx.y * p.b.table_stride;
     const int mask = (1 << p.c.shift) - 1;
-    int ids = -1;
+    const uint32_t at0 = (pc >> 2) * 16384 + km_at(row0, 2 * (pc & 3)), at1 = (pc >> 2) * 16384 + km_at(row0, 2 * (pc & 3) + 1);
+    // blocks of 16 tokens a lane, of the tile being put and of the next one: every load has a tile's time to arrive (nothing looks at an
+    // id before it is used)
+    constexpr int kNone = -2147483647 - 1;
     auto look_up = [&](int j) {
       const int key = k0 + kKmKeys * j + 16 * lane;
-      ids = -1;
-      if (lane < kKmKeys / 16 && key < k1) {
-        ids = __ldg(table + (key >> p.c.shift));
-        if (ids < 0 || ids >= p.c.n_blocks) { ids = -1; atomicCAS(p.status, 0, kDevBadBatch); }
-      }
+      return lane < kKmKeys / 16 && key < k1 ? __ldg(table + (key >> p.c.shift)) : kNone;
     };
-    uint4 r[kPer];
-    auto load = [&](const uint8_t* codes, int j) {
+    auto load = [&](uint4 (&r)[kPer], const uint8_t* codes, int ids, int j) {
+      // head of the block, in units of 1024 bytes (a block of a head is 1024 at least)
+      const uint32_t head = ids < 0 ? 0xFFFFFFFFu : (uint32_t)(((((uint64_t)ids * p.c.heads + kvh) << p.c.shift) * D) >> 10);
+      const int rows = sq.len - (k0 + kKmKeys * j);    // rows behind the last token hold anything
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
-        const int row = row0 + i * (128 / kPer), key = k0 + kKmKeys * j + row;
-        const int id = __shfl_sync(0xffffffffu, ids, row >> 4);
+        const int row = row0 + i * kRows;
+        const uint32_t h = __shfl_sync(0xffffffffu, head, row >> 4);
         r[i] = make_uint4(0, 0, 0, 0);
-        if (id >= 0 && key < sq.len)                   // rows behind the last token hold anything
-          r[i] = __ldg(reinterpret_cast<const uint4*>(codes + ((((size_t)id * p.c.heads + kvh) << p.c.shift) + (key & mask)) * D) + pc);
+        if (h != 0xFFFFFFFFu && row < rows) r[i] = __ldg(reinterpret_cast<const uint4*>(codes + ((uint64_t)h << 10) + (row & mask) * D) + pc);
       }
     };
-    auto put = [&](uint8_t* dst) {
+    auto put = [&](uint8_t* dst, const uint4 (&r)[kPer]) {
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
-        const int row = row0 + i * (128 / kPer), j0 = 2 * (pc & 3), odd = pc >> 2;       // D 128: the upper half's lanes begin with the odd chunk
-        const uint4 lo = make_uint4(kv8_half2(r[i].x), kv8_half2(r[i].x >> 16), kv8_half2(r[i].y), kv8_half2(r[i].y >> 16));
-        const uint4 hi = make_uint4(kv8_half2(r[i].z), kv8_half2(r[i].z >> 16), kv8_half2(r[i].w), kv8_half2(r[i].w >> 16));
-        uint8_t* q = dst + (pc >> 2) * 16384;
-        *reinterpret_cast<uint4*>(q + km_at(row, j0 + odd)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(q + km_at(row, j0 + 1 - odd)) = odd ? lo : hi;
+        *reinterpret_cast<uint4*>(dst + at0 + i * kRows * 128) = make_uint4(kv8_half2(r[i].x), kv8_half2(r[i].x >> 16), kv8_half2(r[i].y), kv8_half2(r[i].y >> 16));
+        *reinterpret_cast<uint4*>(dst + at1 + i * kRows * 128) = make_uint4(kv8_half2(r[i].z), kv8_half2(r[i].z >> 16), kv8_half2(r[i].w), kv8_half2(r[i].w >> 16));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     };
-    look_up(0);
-    load(p.c.k, 0);
-    for (int j = 0; j < n; j++) {
+    const bool scales = warp == S::kSoft;
+    uint4 rk[kPer], rv[kPer];
+    int ids = -1, next = look_up(0);
+    float ks = 0.f, vs = 1.f;
+    // round j: tile j from registers into shared memory, tile j + 1 into the registers
+#pragma unroll 1
+    for (int j = -1; j < n; j++) {
       const int s = j & 1;
-      if (!wait(&hd->kempty[s], (j >> 1) ^ 1, kDevWaitEmpty)) break;
-      put(kmem + s * S::kBytes);
-      if (lane == 0) mbar_arrive(&hd->kfull[s]);
-      load(p.c.v, j);
-      float4 f = make_float4(0.f, -INFINITY, 0.f, 0.f);
-      if (warp == S::kSoft && ids >= 0) {
-        f.x = __ldg(p.c.ks + (size_t)ids * p.c.heads + kvh);
-        const int e = kv8_exp(__ldg(p.c.vs + (size_t)ids * p.c.heads + kvh));
-        f.y = (float)e; f.z = kv8_pow2(-e);
+      const bool more = j + 1 < n;
+      if (j >= 0) {
+        if (!wait(&hd->kempty[s], (j >> 1) ^ 1, kDevWaitEmpty)) break;
+        put(kmem + s * S::kBytes, rk);
+        if (lane == 0) mbar_arrive(&hd->kfull[s]);
       }
-      if (!wait(&hd->vempty[s], (j >> 1) ^ 1, kDevWaitEmpty)) break;     // with it the scales of two tiles ago have been used
-      if (warp == S::kSoft && lane < kKmKeys / 16) hd->sc[s][lane] = f;
-      put(vmem + s * S::kBytes);
-      if (lane == 0) mbar_arrive(&hd->vfull[s]);
-      if (j + 1 < n) { look_up(j + 1); load(p.c.k, j + 1); }
+      if (more) {
+        if (next < 0 || next >= p.c.n_blocks) {
+          if (next != kNone) atomicCAS(p.status, 0, kDevBadBatch);
+          next = -1;
+        }
+        load(rk, p.c.k, next, j + 1);
+      }
+      if (j >= 0) {
+        if (!wait(&hd->vempty[s], (j >> 1) ^ 1, kDevWaitEmpty)) break;     // with it the scales of two tiles ago have been used
+        if (scales && lane < kKmKeys / 16) {
+          const int e = kv8_exp(vs);
+          hd->sc[s][lane] = ids < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(ks, (float)e, kv8_pow2(-e), 0.f);
+        }
+        put(vmem + s * S::kBytes, rv);
+        if (lane == 0) mbar_arrive(&hd->vfull[s]);
+      }
+      if (more) {
+        load(rv, p.c.v, next, j + 1);
+        if (scales && next >= 0) {
+          ks = __ldg(p.c.ks + (size_t)next * p.c.heads + kvh);
+          vs = __ldg(p.c.vs + (size_t)next * p.c.heads + kvh);
+        }
+        ids = next;
+        next = j + 2 < n ? look_up(j + 2) : kNone;
+      }
     }
-  } else if ((warp >> 2) < nt) {
+  } else if (warp < S::kSoft && (warp >> 2) < nt) {
     // ------------------------------------------------------------------ weights: a row a thread
     const int t = warp >> 2, tr = tid & 127, row = m0 + t * kKmRows + tr;
     const bool live = row < R;
     const int tok = min(row, R - 1) / p.G, head = kvh * p.G + min(row, R - 1) % p.G, pos = sq.len - sq.n + tok;
     const int w0 = m0 + t * kKmRows + (warp & 3) * 32, w1 = min(w0 + 31, R - 1);
     const int all_hi = min(k1, sq.len - sq.n + min(w0, R - 1) / p.G + 1), all_lo = p.window ? sq.len - sq.n + w1 / p.G - p.window + 1 : 0;
-    float f0;                                          // logit in binary exponents = product * f0 * key scale
     {
-      const T* src = static_cast<const T*>(p.q) + (sq.row + tok) * p.q_stride + (int64_t)head * D;
-      float top = 0.f, v[8];
-#pragma unroll 4
-      for (int c = 0; c < D / 8; c++) {
-        Elems<T>::load(src + 8 * c, p.q_vec, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i]));
-      }
-      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -60), 120);
-      const float inv = p.scale < 0.f ? -kv8_pow2(-e) : kv8_pow2(-e);
-      f0 = kv8_pow2(e) * fabsf(p.scale) * kLog2e;
+      // the warp's 32 rows, D / 8 lanes a row: their largest, then halves.  A logit in binary exponents is product * f0 * key scale
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
       uint8_t* dst = qs_mem + t * S::kTerms * S::kBytes;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; c++) {
-        Elems<T>::load(src + 8 * c, p.q_vec, v);
-        uint32_t hi[4], lo[4];
+      const int c = lane % kLanes, dq = kAtOnce / p.G, dr = kAtOnce % p.G;
+      constexpr int kBatch = TWO ? 4 : 8;              // rows requested at once
+      int rr = w0 + lane / kLanes, tk = rr / p.G, hh = rr - tk * p.G;        // row, token, head of the group
+#pragma unroll 1
+      for (int i0 = 0; i0 < kLanes; i0 += kBatch) {
+        typename Elems<T>::Raw x[kBatch] = {};
+        const T* src[kBatch];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float a = live ? v[2 * i] * inv : 0.f, b = live ? v[2 * i + 1] * inv : 0.f;
-          hi[i] = km_pack(a, b);
-          if (TWO) {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-            lo[i] = km_pack(a - h.x, b - h.y);
+        for (int i = 0; i < kBatch; i++) {
+          src[i] = rr < R ? static_cast<const T*>(p.q) + (sq.row + tk) * p.q_stride + (kvh * p.G + hh) * D + 8 * c : nullptr;
+          rr += kAtOnce; tk += dq; hh += dr;
+          if (hh >= p.G) { hh -= p.G; tk++; }
+          if (p.q_vec && src[i]) x[i] = Elems<T>::raw(src[i]);
+        }
+        if (!p.q_vec) {
+#pragma unroll
+          for (int i = 0; i < kBatch; i++) {
+            T* y = reinterpret_cast<T*>(&x[i]);
+            if (src[i])
+#pragma unroll
+              for (int k = 0; k < 8; k++) y[k] = src[i][k];
           }
         }
-        uint8_t* q = dst + (c >> 3) * 16384 + km_at(tr, c & 7);
-        *reinterpret_cast<uint4*>(q) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (TWO) *reinterpret_cast<uint4*>(q + S::kBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+          const int r = (i0 + i) * kAtOnce + lane / kLanes;
+          float v[8], top = 0.f;
+          Elems<T>::open(x[i], v);
+#pragma unroll
+          for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -60), 120);
+          const float inv = p.scale < 0.f ? -kv8_pow2(-e) : kv8_pow2(-e);
+          if (c == 0) hd->f0[t * 128 + (warp & 3) * 32 + r] = kv8_pow2(e) * fabsf(p.scale) * kLog2e;
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            hi[k] = km_pack(v[2 * k] * inv, v[2 * k + 1] * inv);
+            if (TWO) {
+              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+              lo[k] = km_pack(v[2 * k] * inv - h.x, v[2 * k + 1] * inv - h.y);
+            }
+          }
+          uint8_t* q = dst + (c >> 3) * 16384 + km_at((warp & 3) * 32 + r, c & 7);
+          *reinterpret_cast<uint4*>(q) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (TWO) *reinterpret_cast<uint4*>(q + S::kBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&hd->qfull);
     }
+    const float f0 = hd->f0[t * 128 + tr];
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + t * 128, to = tmem + lanes + S::kO + t * D;
+    const int first = p.window ? max(0, pos - p.window + 1) : 0, last = min(k1 - 1, pos);      // keys that the row sees
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n; j++) {
       const int s = j & 1, base = k0 + kKmKeys * j;
-      ok = wait(&hd->sfull[t], j, kDevWaitFull) && wait(&hd->vfull[s], j >> 1, kDevWaitFull);
+      ok = wait(&hd->sfull[t], j, kDevWaitFull) && wait(&hd->vfull[s], j >> 1, kDevWaitFull);     // the tile's scales come with its values
       if (!ok) break;
       __syncwarp();
       ts_fence_after();
       const bool cut = base + kKmKeys > all_hi || base < all_lo;
-      auto seen = [&](int col) {
-        const int key = base + col;
-        return key < k1 && key <= pos && (!p.window || key > pos - p.window);
-      };
-      uint32_t a[2][16];
-      // ---- the largest exponent
-      float top = -INFINITY;
-      ts_ld16(ts, a[0]);
-#pragma unroll
-      for (int c = 0; c < kKmKeys / 16; c++) {
-        ts_wait_ld();
-        if (c + 1 < kKmKeys / 16) ts_ld16(ts + 16 * (c + 1), a[(c + 1) & 1]);
-        const float4 sc = hd->sc[s][c];
-        const float f = f0 * sc.x;
-        float x = -INFINITY;
-        if (cut) {
+      float mm = m == -INFINITY ? 0.f : m;
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {   // no reference yet: the tile's largest exponent (that of its first 16 keys had to move later)
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kKmKeys / 16; c++) {
+          uint32_t a[16];
+          ts_ld16(ts + 16 * c, a);
+          ts_wait_ld();
+          const float4 sc = hd->sc[s][c];
+          const float f = f0 * sc.x;
+          const int hi = cut ? last - base - 16 * c : 16, lo = cut ? first - base - 16 * c : 0;
 #pragma unroll
           for (int i = 0; i < 16; i++)
-            if (seen(16 * c + i)) x = fmaxf(x, fmaf(__uint_as_float(a[c & 1][i]), f, sc.y));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i++) x = fmaxf(x, __uint_as_float(a[c & 1][i]));
-          x = fmaf(x, f, sc.y);
+            if (i <= hi && i >= lo) top = fmaxf(top, fmaf(__uint_as_float(a[i]), f, sc.y));
+          __syncwarp();
         }
-        top = fmaxf(top, x);
-        __syncwarp();
+        if (m == -INFINITY) m = top;
+        mm = m == -INFINITY ? 0.f : m;
       }
-      if (__any_sync(0xffffffffu, top > m + 8.f)) {
-        const float nm = top > m + 8.f ? top : m, f = nm == -INFINITY ? 1.f : km_exp2(m - nm);
-        m = nm; l *= f;
-        if (j) {
+      // ---- weights, 64 keys at a time, into columns of products that have been read.  The reference stays unless the weights of 16 keys
+      // sum to more than 2^15 (a half holds each of them then): it moves up by a whole number, what has been summed against the old one is
+      // scaled, and the 64 weights are made again
+      float sum = 0.f;
+      bool lost = false;
+      int tries = 0;
 #pragma unroll 1
-          for (int c = 0; c < D / 16; c++) {
-            ts_ld16(to + 16 * c, a[0]);
-            ts_wait_ld();
+      for (int c = 0; c < kKmKeys / 16;) {             // (unrolled, its code no longer stays in the instruction cache)
+        uint32_t w[4][16];
+        float part[4];
 #pragma unroll
-            for (int i = 0; i < 16; i++) a[0][i] = __float_as_uint(__uint_as_float(a[0][i]) * f);
-            ts_st16(to + 16 * c, a[0]);
+        for (int h = 0; h < 4; h++) ts_ld16(ts + 16 * (c + h), w[h]);
+        ts_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+          const float4 sc = hd->sc[s][c + h];
+          const uint64_t f = km_two(f0 * sc.x, f0 * sc.x), b = km_two(sc.y - mm, sc.y - mm);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float x, y;
+            km_apart(km_fma2(km_two(__uint_as_float(w[h][i]), __uint_as_float(w[h][i + 1])), f, b), x, y);
+            w[h][i] = __float_as_uint(x); w[h][i + 1] = __float_as_uint(y);
           }
         }
-      }
-      const float mm = m == -INFINITY ? 0.f : m;
-      // ---- weights, in place of the products
-      ts_ld16(ts, a[0]);
+        if (cut) {
+          const int hi = last - base - 16 * c, lo = first - base - 16 * c;
 #pragma unroll
-      for (int c = 0; c < kKmKeys / 16; c += 2) {
-        uint32_t hi[16], lo[16];
+          for (int i = 0; i < 64; i++)
+            if (i > hi || i < lo) w[i >> 4][i & 15] = 0xFF800000u;
+          __syncwarp();
+        }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          ts_wait_ld();
-          if (c + h + 1 < kKmKeys / 16) ts_ld16(ts + 16 * (c + h + 1), a[(h + 1) & 1]);
-          const float4 sc = hd->sc[s][c + h];
-          const float f = f0 * sc.x, b = sc.y - mm;
-          float w[16], sum = 0.f;
+        for (int h = 0; h < 4; h++) {
+          uint64_t x[2] = {0, 0};
 #pragma unroll
-          for (int i = 0; i < 16; i++) w[i] = fmaf(__uint_as_float(a[h][i]), f, b);
-          if (cut) {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-              if (!seen(16 * (c + h) + i)) w[i] = -INFINITY;
-            __syncwarp();
+          for (int i = 0; i < 16; i += 2) {
+            float u = __uint_as_float(w[h][i]), v = __uint_as_float(w[h][i + 1]);
+            if (!TWO && (i & 6) == 6) km_exp2_fma(u, v);       // a quarter of them beside the others (F32 keeps its two units' accuracy)
+            else { u = km_exp2(u); v = km_exp2(v); }
+            w[h][i] = __float_as_uint(u); w[h][i + 1] = __float_as_uint(v);
+            x[i >> 1 & 1] = km_add2(x[i >> 1 & 1], km_two(u, v));
           }
+          float y, z;
+          km_apart(km_add2(x[0], x[1]), y, z);
+          part[h] = y + z;
+        }
+        const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        if (__any_sync(0xffffffffu, most > 32768.f && !lost)) {
+          // to the next power of two above the sum, or, where that is beyond 32 bits, to the largest exponent.  A row whose products
+          // are infinite has none, and beyond 2^35 exponents are too coarse for one: after four times its weights stay what they are
+          float up = most > 32768.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) : 0.f;
+          if (__any_sync(0xffffffffu, up > 128.f)) {
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+              ts_ld16(ts + 16 * (c + k), w[0]);
+              ts_wait_ld();
+              const float4 sc = hd->sc[s][c + k];
 #pragma unroll
-          for (int i = 0; i < 16; i++) { w[i] = km_exp2(w[i]); sum += w[i]; }
-          l = fmaf(sum, sc.z, l);
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            hi[8 * h + i] = km_pack(w[2 * i], w[2 * i + 1]);
-            if (TWO) {
-              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hi[8 * h + i]));
-              lo[8 * h + i] = km_pack(w[2 * i] - x.x, w[2 * i + 1] - x.y);
+              for (int i = 0; i < 16; i++) {
+                const int key = base + 16 * (c + k) + i;
+                if (!cut || (key >= first && key <= last)) top = fmaxf(top, fmaf(__uint_as_float(w[0][i]), f0 * sc.x, sc.y - mm));
+              }
+              __syncwarp();
+            }
+            if (up > 128.f) {
+              lost = !(top < INFINITY);
+              up = lost ? 0.f : ceilf(top);
             }
           }
+          if (++tries == 4) lost = true;
+          const float f = km_exp2(-up);
+          m += up; mm = m; l *= f; sum *= f;
+          if (j | c) {
+            // the sums so far: with the first 64 weights of this tile, once their products are there
+            if (c) ok = wait(&hd->ahalf[t], j, kDevWaitFull);
+            if (!ok) break;
+            __syncwarp();
+            ts_fence_after();
+#pragma unroll 1
+            for (int k = 0; k < D / 16; k++) {
+              ts_ld16(to + 16 * k, w[0]);
+              ts_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; i++) w[0][i] = __float_as_uint(__uint_as_float(w[0][i]) * f);
+              ts_st16(to + 16 * k, w[0]);
+            }
+          }
+          ts_wait_st();
+          continue;
         }
-        // the products of columns below 16 c + 32 have been read: [8 c, 8 c + 16) are free
-        ts_st16(ts + 8 * c, hi);
-        if (TWO) ts_st16(tmem + lanes + S::kLow + 8 * c, lo);
+#pragma unroll
+        for (int h = 0; h < 4; h++) sum = fmaf(part[h], hd->sc[s][c + h].z, sum);
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float u = __uint_as_float(w[h + (i >> 3)][2 * i & 15]), v = __uint_as_float(w[h + (i >> 3)][(2 * i & 15) + 1]);
+            hi[i] = km_pack(u, v);
+            if (TWO) {
+              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+              lo[i] = km_pack(u - y.x, v - y.y);
+            }
+          }
+          ts_st16(ts + 8 * (c + h), hi);
+          if constexpr (TWO) ts_st16(tmem + lanes + S::kLow + 8 * (c + h), lo);
+        }
+        ts_wait_st();
+        ts_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&hd->pfull[t][c >> 2]);
+        c += 4;
+        tries = 0;
       }
-      ts_wait_st();
-      ts_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&hd->pfull[t]);
+      if (!ok) break;
+      l += sum;
     }
     if (ok) ok = wait(&hd->ofull[t], 0, kDevWaitFull);
     if (ok) {
@@ -382,7 +521,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
   }
   ts_fence_before();
   __syncthreads();
-  if (warp == S::kWarps - 1) {
+  if (warp == S::kMma) {
     ts_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }

@@ -372,3 +372,47 @@ def test_refusals_that_need_a_device():
     with pytest.raises(_lib.MsbError):
         kv8.attn_scratch(cache, batch, 15)
     e.wait()
+
+
+@pytest.mark.parametrize("dt", ("f32", "bf16"))
+@pytest.mark.parametrize("n", (1, 64))
+def test_attention_where_the_largest_logit_comes_late_or_is_huge(n, dt):
+    """Logits that grow along the keys by far more than a weight may grow before the sums are rescaled, and ones of 1e6 and more."""
+    from macseek_b200 import kv8
+    D = 64
+    c = R.Case([(n, 700)], 1, D, 64, seed=4)
+    c.k.fill_(0x38)                                                   # ones
+    cache, batch, e = c.cache(), c.batch(), enc()
+    q = torch.full((c.rows, 4, D), 1.0, dtype=R.DT[dt], device="cuda") * torch.tensor([1.0, -1.0, 0.5, 0.0], device="cuda", dtype=R.DT[dt])[None, :, None]
+    for first, factor in ((1, 2.0), (2.0 ** 20, 1.0), (1, 8.0)):
+        for b in range(11):                                           # key scales: a block's logits are first * factor^b * 64 * scale
+            c.ks[c.table_host[0, b]] = first * factor ** b
+        out = torch.zeros_like(q)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 4))
+        e.wait()
+        assert not torch.isnan(out).any()
+        # a row of equal keys inside each block: the average over the last block it sees (positive), the first (negative) or all (zero)
+        ref, _ = R.attn_ref(c, q, out, D ** -0.5)
+        half, _ = R.half_step(q.dtype)
+        # equal keys have equal weights: what is left is the weights' rounding, their sum and the output's
+        tol = 4.0 * (2.0 ** -11 + 700 / 8 * 2.0 ** -23 + 2.0 ** -20 + 700 * 2.0 ** -25 + half)
+        assert float((out.double() - ref).abs().max()) <= tol * float(c.held(0, "v").abs().max()) / 4
+
+
+def test_attention_of_what_is_not_a_number_ends():
+    """NaN, infinite and absurdly large queries: the call ends, and rows beside them are not touched by them."""
+    from macseek_b200 import kv8
+    for n in (1, 80):
+        c = R.Case([(n, 300), (n, 200)], 1, 64, 16, seed=6)
+        q = c.randn(c.rows, 4, 64)
+        q[0, 0, 3], q[0, 1, 5], q[0, 2] = float("nan"), float("inf"), 1e38
+        cache, batch, e = c.cache(), c.batch(), enc()
+        out = torch.zeros_like(q)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 4))
+        e.wait()
+        assert torch.isnan(out[0, 0]).all()
+        q[0, :3] = 0
+        ref, tol = R.attn_ref(c, q, out, 0.125)
+        bad = (out.double() - ref).abs() > tol
+        bad[0, :3] = False
+        assert not bad.any()
