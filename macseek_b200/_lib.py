@@ -38,6 +38,10 @@ def host():
         raise ImportError("libmacseek_b200_host.so was built for %s, this is %s: run `python -m macseek_b200.build`"
                           % (h.msb_host_built_for().decode(), target))
     h.msb_slot_addresses.argtypes = [C.py_object, C.py_object, C.c_int64, C.c_void_p]
+    o, p, i, d = C.py_object, C.c_void_p, C.c_int, C.c_double
+    h.msb_host_kv8_rows.argtypes = [o, o, p, p, i, p, p]
+    h.msb_host_kv8_attn.argtypes = [o, o, o, o, p, p, i, d, i, p, p]
+    h.msb_host_head_norm_rope.argtypes = [o, o, o, o, d, o, o, o, o, i, i, i, p, p]
     return h
 
 
@@ -173,3 +177,8 @@ lib.msb_kv8_attn_scratch_bytes.restype = C.c_size_t
 lib.msb_kv8_attn_scratch_bytes.argtypes = [C.POINTER(Kv8CacheC), C.POINTER(Kv8BatchC), _i]
 lib.msb_kv8_attn.argtypes = [C.POINTER(Kv8CacheC), C.POINTER(Kv8BatchC), _i, _vp, _i64, _i, _f, _i, _vp, _vp, _i64, _vp,
                              C.c_size_t, _vp]
+
+
+def address(fn):
+    """Address of an entry point, for host code that calls it."""
+    return C.cast(fn, C.c_void_p).value

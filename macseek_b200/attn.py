@@ -144,32 +144,29 @@ def encode_compress(e: Enc, s: DecodeState, c_kv, c_gate, c_norm, wk_bf16, k_nor
                                      ptr(s.ikey), e.handle))
 
 
+_NORM_ROPE = _lib.address(_lib.lib.msb_head_norm_rope)
+
+
 def encode_head_norm_rope(e: Enc, q, k, q_w, k_w, eps, cs, pos, q_out, k_out, rot_first=0, halves=False):
     """RMSNorm of every query and key head (q [n][heads][D], k [n][kv_heads][D]; either may be None) and the rotation of dims
     [rot_first, rot_first + 2 cs.shape[1]) by position pos [n] (int32; negative: a padding row, left out) in one pass, into
     q_out, k_out (may be q, k).  cs: F32 [positions][pairs][2] as make_rope_table's; pairs are neighbouring dims, or with
     halves dims half the rotated width apart.  (No counterpart in the reference: encode_kv_window has one head.)"""
-    x = k if q is None else q
-    n, _, D = x.shape
-    dev = x.device
-    heads, strides, types = [], [], set()
-    for name, a, w, b in (("q", q, q_w, q_out), ("k", k, k_w, k_out)):
-        if a is None:
-            heads.append(0)
-            strides.append((0, 0))
-            continue
-        heads.append(a.shape[1])
-        for t in (a, b):
-            types.add(kv8._rows(name, t, n, a.shape[1], D, dev))
-        strides.append((kv8._stride(a), kv8._stride(b)))
-        kv8._want(w is None or (w.device == dev and w.dtype == torch.float32 and w.numel() == D and w.is_contiguous()),
-                  "%s_w must be contiguous float32 [%d]" % (name, D))
-    kv8._want(len(types) == 1, "q, k and their outputs must be of one type")
-    kv8._want(pos.device == dev and pos.dtype == torch.int32 and pos.numel() == n and pos.is_contiguous(), "pos must be contiguous int32 [%d]" % n)
-    kv8._want(cs.device == dev and cs.dtype == torch.float32 and cs.dim() == 3 and cs.shape[2] == 2 and cs.is_contiguous(),
-              "cs must be contiguous float32 [positions][pairs][2]")
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with kv8._on_stream(e, dev):
-        _lib.check(_lib.lib.msb_head_norm_rope(types.pop(), p(q), heads[0], strides[0][0], p(q_w), p(k), heads[1], strides[1][0], p(k_w), n, D,
-                                               eps, p(cs), p(pos), cs.shape[0], 2 * cs.shape[1], rot_first, int(halves), p(q_out),
-                                               strides[0][1], p(k_out), strides[1][1], e.handle))
+    dev = cs.device
+    rc = kv8._call(e, dev, _lib.host().msb_host_head_norm_rope, q, k, q_w, k_w, eps, cs, pos, q_out, k_out, dev.index, rot_first, int(halves),
+                   _NORM_ROPE)
+    if rc > 0:                     # not plainly right: say why
+        x = k if q is None else q
+        kv8._want(x is not None and x.dim() == 3, "head_norm_rope: q or k must be [n][heads][D]")
+        n, _, D = x.shape
+        types = set()
+        for name, a, w, b in (("q", q, q_w, q_out), ("k", k, k_w, k_out)):
+            if a is not None:
+                types |= {kv8._rows(name, a, n, a.shape[1], D, dev), kv8._rows(name + "_out", b, n, a.shape[1], D, dev)}
+            kv8._want(w is None or (w.device == dev and w.dtype == torch.float32 and w.numel() == D and w.is_contiguous()),
+                      "%s_w must be contiguous float32 [%d]" % (name, D))
+        kv8._want(len(types) == 1, "q, k and their outputs must be of one type")
+        kv8._want(pos is not None and pos.device == dev and pos.dtype == torch.int32 and pos.numel() == n and pos.is_contiguous(),
+                  "pos must be contiguous int32 [%d]" % n)
+        kv8._want(False, "cs must be contiguous float32 [positions][pairs][2]")
+    _lib.check(rc)

@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libmacseek_b200.so")
-HOST_SRC = os.path.join(CSRC, "slot_addresses.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("slot_addresses.cpp", "kv8_calls.cpp")]
 HOST_LIB = os.path.join(HERE, "libmacseek_b200_host.so")    # what reads PyTorch tensors
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -41,7 +41,7 @@ def _compile(src):
 
 def _host_stale(target):
     """The sources changed, or another PyTorch or Python is installed than the library was built for (it says which)."""
-    if _stale(HOST_LIB, [HOST_SRC, os.path.abspath(__file__)]):
+    if _stale(HOST_LIB, HOST_SRCS + [os.path.join(HERE, "..", "include", "macseek_b200.h"), os.path.abspath(__file__)]):
         return True
     with open(HOST_LIB, "rb") as f:
         return target.encode() + b"\0" not in f.read()
@@ -63,7 +63,7 @@ def _build_host():
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     subprocess.check_call(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(),
                            '-DMSB_BUILT_FOR="%s"' % target]
-                          + inc + [HOST_SRC, "-o", HOST_LIB, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10"])
+                          + inc + HOST_SRCS + ["-o", HOST_LIB, "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10"])
 
 
 def build(verbose=False, jobs=None):

@@ -1,102 +1,147 @@
 // RMSNorm of every query and key head and the rotation by position, in one pass over the projections' rows.
 //   y = x * rsqrt(mean(x^2) + eps) * w ;  (a, b) -> (a c - b s, a s + b c) for the pairs of dims [first, first + rot)
-// Bound by memory: each value is read and written once.  Eight elements per lane, so a head of 64 / 128 / 256 dims is 8 / 16 / 32 lanes
-// and a warp has 4 / 2 / 1 heads; a row's (cos, sin) factors are loaded once per lane and used for all heads of the token.
+// Each value is read and written once.  Eight elements per lane, so a head of 64 / 128 / 256 dims is 8 / 16 / 32 lanes and a warp has
+// 4 / 2 / 1 heads at a time; the gains are multiplied into the token's (cos, sin) factors, which stay in a lane's registers for all its
+// heads.  A block is one warp with all heads of a token: what a token costs before its first head is then spread over all of them
+// (4096 tokens with 64 + 8 heads of 128, bf16: 38.6 us = 3.97 TB/s, bound by issue and by the latency of each group of loads).
 #include <algorithm>
 #include "kv8.cuh"
 
 namespace msb {
 
+struct NormRopeSide {             // the query heads, or the key heads
+  const void* in;
+  void* out;
+  const float* w;
+  int64_t in_stride, out_stride;
+  int heads, vec;
+};
 struct NormRopeParams {
-  const void *q, *k;
-  void *q_out, *k_out;
-  const float *q_w, *k_w, *cs;
+  NormRopeSide q, k;
+  const float* cs;
   const int* pos;
-  int64_t q_stride, k_stride, q_out_stride, k_out_stride;
-  int q_heads, k_heads, D, rot, first, halves, n_pos, per_block;
-  int q_vec, k_vec;
+  int D, rot, first, halves, n_pos, per_block, cs_vec, w_vec;
   float eps;
   int* status;
 };
 
-constexpr int kNrThreads = 256;
+constexpr int kNrThreads = 32;      // (of 64: 40.0 us, of 128: 49.1 for the prompt above; a chunk of 999 tokens 5.8 and 7.8)
 
 // LANES lanes a head (a power of two >= D / 8)
 template <class T, int LANES>
 __global__ void __launch_bounds__(kNrThreads) head_norm_rope_kernel(const NormRopeParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kGroups = kNrThreads / LANES;
-  const int lane = threadIdx.x & 31, l = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  constexpr int kGroups = kNrThreads / LANES, kWarp = 32 / LANES;      // heads of a block, of a warp
+  typedef typename Elems<T>::Raw Raw;
+  constexpr int kHeads = 4;                               // heads of a group of lanes that are under way at a time
+  const int lane = threadIdx.x & 31, l = threadIdx.x % LANES, group = threadIdx.x / LANES, warp0 = group / kWarp * kWarp;
   const int64_t row = blockIdx.x;
+  const int d = 8 * l;
+  const bool live = d < p.D;
   const int pos = __ldg(p.pos + row);
   if (pos < 0) return;                                    // a padding row
   if (pos >= p.n_pos) {
     if (threadIdx.x == 0) atomicCAS(p.status, 0, kDevBadBatch);
     return;
   }
-  const int d = 8 * l;
-  const bool live = d < p.D, turned = live && d >= p.first && d < p.first + p.rot;
-  // this lane's factors: of its four pairs, or of its eight dims' pairs (halves)
-  float c[8], s[8];
+  const bool turned = live && d >= p.first && d < p.first + p.rot;
   const int half = p.rot >> 1;
   const bool upper = p.halves && d - p.first >= half;     // the second member of its pairs
-  if (turned) {
-    const float* f = p.cs + (int64_t)pos * p.rot + (p.halves ? 2 * (d - p.first - (upper ? half : 0)) : d - p.first);
+  const int partner = turned ? lane + (upper ? -(half >> 3) : half >> 3) : lane, other = p.halves ? d + (upper ? -half : half) : d;
+  const float inv_d = 1.f / (float)p.D;
+  // this block's share of the query heads, then of the key heads
+#pragma unroll 1
+  for (int side = 0; side < 2; side++) {
+    const NormRopeSide& sd = side ? p.k : p.q;
+    const int from = (int)blockIdx.y * p.per_block - (side ? p.q.heads : 0), h0 = max(from, 0), h1 = min(from + p.per_block, sd.heads);
+    if (h0 >= h1) continue;
+    const bool vec = sd.vec;
+    const float* w = sd.w;
+    const T* x = static_cast<const T*>(sd.in) + row * sd.in_stride + d;
+    T* y = static_cast<T*>(sd.out) + row * sd.out_stride + d;
+    Raw raw[kHeads];
+    auto load = [&](int hb) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (i < 4 || p.halves) { c[i] = __ldg(f + 2 * i); s[i] = __ldg(f + 2 * i + 1); }
-  }
-  const int partner = lane + (upper ? -(half >> 3) : half >> 3);
-  const int h0 = blockIdx.y * p.per_block, h1 = min(h0 + p.per_block, p.q_heads + p.k_heads);
-  for (int hb = h0; hb < h1; hb += kGroups) {             // the same count in every warp: the shuffles below are whole
-    const int h = hb + group;
-    const bool mine = live && h < h1, key = h >= p.q_heads;
-    const int hh = key ? h - p.q_heads : h;
-    const bool vec = key ? p.k_vec : p.q_vec;
-    const float* w = key ? p.k_w : p.q_w;
-    float x[8], g[8];
+      for (int i = 0; i < kHeads; i++) {
+        const int h = hb + i * kGroups;
+        raw[i] = {};
+        if (live && h < h1) raw[i] = vec ? Elems<T>::raw(x + h * p.D) : Elems<T>::gather(x + h * p.D);
+      }
+    };
+    load(h0 + group);
+    // with the gains in the factors: y_i = r (x_i a_i + o_i b_i), o_i the other member of the pair (of what is not turned: itself, times 0)
+    float a[8], b[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) { x[i] = 0.f; g[i] = 1.f; }
-    if (mine) {
-      Elems<T>::load(static_cast<const T*>(key ? p.k : p.q) + row * (key ? p.k_stride : p.q_stride) + (int64_t)hh * p.D + d, vec, x);
-      if (w) {
+    for (int i = 0; i < 8; i++) { a[i] = 1.f; b[i] = 0.f; }
+    if (w && live) Elems<float>::load(w + d, p.w_vec, a);
+    if (turned) {
+      float g[8], t[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) g[i] = __ldg(w + d + i);
+      for (int i = 0; i < 8; i++) g[i] = a[i];
+      if (w && p.halves) Elems<float>::load(w + other, p.w_vec, g);
+      const float* f = p.cs + (int64_t)pos * p.rot + (p.halves ? 2 * (d - p.first - (upper ? half : 0)) : d - p.first);
+      Elems<float>::load(f, p.cs_vec, t);
+      if (p.halves) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { a[i] *= t[2 * i]; b[i] = g[i] * (upper ? t[2 * i + 1] : -t[2 * i + 1]); }
+        Elems<float>::load(f + 8, p.cs_vec, t);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { a[4 + i] *= t[2 * i]; b[4 + i] = g[4 + i] * (upper ? t[2 * i + 1] : -t[2 * i + 1]); }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          a[i] *= t[i]; a[i + 1] *= t[i];
+          b[i] = -g[i + 1] * t[i + 1]; b[i + 1] = g[i] * t[i + 1];
+        }
       }
     }
-    float ss = 0.f;
+    uint64_t a2[4], b2[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < 4; i++) { a2[i] = kv8_two(a[2 * i], a[2 * i + 1]); b2[i] = kv8_two(b[2 * i], b[2 * i + 1]); }
+    for (int hb = h0 + group; hb - group + warp0 < h1;) { // whole warps: the shuffles need every lane
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss / (float)p.D + p.eps);
+      for (int i = 0; i < kHeads; i++) {
+        const int h = hb + i * kGroups;
+        if (h - group + warp0 >= h1) break;               // none of the warp's
+        float v[8], o[8];
+        Elems<T>::open(raw[i], v);
+        if (p.halves) {
+          Elems<T>::open(Elems<T>::from_lane(raw[i], partner), o);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = x[i] * r * g[i];
-    if (p.halves) {
+          for (int j = 0; j < 8; j++) o[j] = turned ? v[j ^ 1] : v[j];
+        }
+        uint64_t x2[4], ss = 0;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float o = __shfl_sync(0xffffffffu, x[i], partner & 31);
-        if (turned) x[i] = upper ? fmaf(o, s[i], x[i] * c[i]) : fmaf(x[i], c[i], -(o * s[i]));
+        for (int j = 0; j < 4; j++) {
+          x2[j] = kv8_two(v[2 * j], v[2 * j + 1]);
+          ss = kv8_fma2(x2[j], x2[j], ss);
+        }
+        float sum, rest;
+        kv8_apart(ss, sum, rest);
+        sum += rest;
+#pragma unroll
+        for (int k = LANES / 2; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        const float r = rsqrtf(fmaf(sum, inv_d, p.eps));
+        const uint64_t r2 = kv8_two(r, r);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          kv8_apart(kv8_mul2(r2, kv8_fma2(x2[j], a2[j], kv8_mul2(kv8_two(o[2 * j], o[2 * j + 1]), b2[j]))), v[2 * j], v[2 * j + 1]);
+        if (live && h < h1) Elems<T>::store(y + h * p.D, vec, v);
       }
-    } else if (turned) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = fmaf(a, c[i], -(b * s[i]));
-        x[2 * i + 1] = fmaf(a, s[i], b * c[i]);
-      }
+      hb += kHeads * kGroups;
+      if (hb - group + warp0 < h1) load(hb);
     }
-    if (mine)
-      Elems<T>::store(static_cast<T*>(key ? p.k_out : p.q_out) + row * (key ? p.k_out_stride : p.q_out_stride) + (int64_t)hh * p.D + d, vec, x);
   }
 }
 
 template <class T>
 static int launch_norm_rope(NormRopeParams& p, int n_tokens, cudaStream_t st) {
-  const int lanes = p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, groups = kNrThreads / lanes, heads = p.q_heads + p.k_heads;
-  p.per_block = std::max(groups, n_tokens >= 1024 ? heads : groups);
-  const dim3 grid((unsigned)n_tokens, (unsigned)((heads + p.per_block - 1) / p.per_block));
+  const int lanes = p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, groups = kNrThreads / lanes;
+  // all heads in a block once the tokens alone fill the GPU twice, a head a group of lanes before
+  p.per_block = n_tokens >= 2 * 148 ? p.q.heads + p.k.heads : groups;
+  const dim3 grid((unsigned)n_tokens, (unsigned)((p.q.heads + p.k.heads + p.per_block - 1) / p.per_block));
   auto go = [&](auto kern) { return launch_pdl(kern, grid, dim3(kNrThreads), 0, st, p); };
   MSB_CUDA(lanes == 8 ? go(head_norm_rope_kernel<T, 8>) : lanes == 16 ? go(head_norm_rope_kernel<T, 16>) : go(head_norm_rope_kernel<T, 32>));
   MSB_LAUNCH_CHECK("head_norm_rope");
@@ -122,10 +167,12 @@ int head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, 
                   (rc = kv8_rows_check(k_out, k_out_stride, k_heads, D, elem_type, what, &v[3])))) return rc;
   Tables tb;
   if ((rc = get_tables(&tb))) return rc;
-  p.q = q; p.k = k; p.q_out = q_out; p.k_out = k_out; p.q_w = q_w; p.k_w = k_w; p.cs = cs; p.pos = pos;
-  p.q_stride = q_stride; p.k_stride = k_stride; p.q_out_stride = q_out_stride; p.k_out_stride = k_out_stride;
-  p.q_heads = q_heads; p.k_heads = k_heads; p.D = D; p.rot = rot; p.first = first; p.halves = halves != 0; p.n_pos = n_pos;
-  p.q_vec = v[0] && v[1]; p.k_vec = v[2] && v[3]; p.eps = eps; p.status = tb.status;
+  p.q = NormRopeSide{q, q_out, q_w, q_stride, q_out_stride, q_heads, v[0] && v[1]};
+  p.k = NormRopeSide{k, k_out, k_w, k_stride, k_out_stride, k_heads, v[2] && v[3]};
+  p.cs = cs; p.pos = pos; p.D = D; p.rot = rot; p.first = first; p.halves = halves != 0; p.n_pos = n_pos;
+  p.cs_vec = reinterpret_cast<uintptr_t>(cs) % 16 == 0 && rot % 4 == 0;
+  p.w_vec = (reinterpret_cast<uintptr_t>(q_w) | reinterpret_cast<uintptr_t>(k_w)) % 16 == 0;
+  p.eps = eps; p.status = tb.status;
   return elem_type == F32 ? launch_norm_rope<float>(p, n_tokens, st) : elem_type == F16 ? launch_norm_rope<__half>(p, n_tokens, st)
                                                                                         : launch_norm_rope<__nv_bfloat16>(p, n_tokens, st);
 }

@@ -6,6 +6,7 @@
 // Powers of two: a code moves from one scale to a larger one by its exponent alone, so a block whose largest value grows token by
 // token keeps its older codes' mantissas, and values and codes convert without a rounding of the scale.
 #pragma once
+#include <type_traits>
 #include "msb_common.cuh"
 #include "kv8_index.h"
 #include "../../include/macseek_b200.h"
@@ -43,21 +44,46 @@ template <class F>
 __device__ __forceinline__ int kv8_find(int n, int x, F first) {       // by whole warps
   return kv8_search(n, x, first, [](auto f) { return __ballot_sync(0xffffffffu, f(threadIdx.x & 31)); });
 }
-// Work item `item` (kv8_index.h) and its block's id (-1: not there).
-__device__ __forceinline__ Kv8Item kv8_item(const Kv8Batch& b, const Kv8Cache& c, int item, int* status, int& id) {
-  auto first = [&](int s) { return kv8_first_item(__ldg(b.seq_start + s), s, c.shift); };
-  const int s = kv8_find(b.n_seq, item, first);
-  const Kv8Item it = kv8_item_of(kv8_seq(b, s, status), item - first(s), c.shift);
-  id = -1;
-  if (it.n == 0) return it;
-  id = __ldg(b.table + (size_t)s * b.table_stride + it.blk);
-  if (id < 0 || id >= c.n_blocks) {
-    id = -1;
-    atomicCAS(status, 0, kDevBadBatch);
+// Work item `item` (kv8_index.h): `each` > 0: sequence item / each, its item % each; 0: found among the sequences' first items.  By whole warps.
+__device__ __forceinline__ Kv8Item kv8_item(const Kv8Batch& b, int shift, int each, int item, int* status, int& s) {
+  if (each) {
+    s = item / each;
+    return kv8_item_of(kv8_seq(b, s, status), item - s * each, shift);
   }
-  return it;
+  auto first = [&](int i) { return kv8_first_item(__ldg(b.seq_start + i), i, shift); };
+  s = kv8_find(b.n_seq, item, first);
+  return kv8_item_of(kv8_seq(b, s, status), item - first(s), shift);
+}
+// The block of an item of sequence s (-1: not there).
+__device__ __forceinline__ int kv8_block(const Kv8Batch& b, int n_blocks, int s, const Kv8Item& it, int* status) {
+  const int id = __ldg(b.table + (size_t)s * b.table_stride + it.blk);
+  if (id >= 0 && id < n_blocks) return id;
+  atomicCAS(status, 0, kDevBadBatch);
+  return -1;
 }
 
+// two f32 at a time
+__device__ __forceinline__ uint64_t kv8_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void kv8_apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t kv8_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t kv8_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t kv8_mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ float kv8_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }    // -126 <= e <= 127
 __device__ __forceinline__ int kv8_exp(float scale) {
   return min(max((int)(__float_as_uint(scale) >> 23 & 0xFF) - 127, kKv8MinExp), kKv8MaxExp);
@@ -80,11 +106,39 @@ __device__ __forceinline__ uint32_t kv8_codes4(float a, float b, float c, float 
   return r;
 }
 
+template <class T>
+__device__ __forceinline__ uint32_t kv8_pack2(float a, float b) {
+  if (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 kv8_from_lane(const uint4& v, int lane) {
+  return make_uint4(__shfl_sync(0xffffffffu, v.x, lane), __shfl_sync(0xffffffffu, v.y, lane), __shfl_sync(0xffffffffu, v.z, lane),
+                    __shfl_sync(0xffffffffu, v.w, lane));
+}
 // eight elements of a row; vec: 16-byte aligned (raw: always)
 template <class T> struct Elems;
 template <> struct Elems<float> {
   struct Raw { uint4 a, b; };                                         // eight elements as they lie in memory
   static __device__ __forceinline__ Raw raw(const float* p) { return Raw{reinterpret_cast<const uint4*>(p)[0], reinterpret_cast<const uint4*>(p)[1]}; }
+  static __device__ __forceinline__ Raw from_lane(const Raw& r, int lane) { return Raw{kv8_from_lane(r.a, lane), kv8_from_lane(r.b, lane)}; }
+  static __device__ __forceinline__ Raw gather(const float* p) {       // not aligned
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = __float_as_uint(p[i]);
+    return Raw{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
+  }
+  static __device__ __forceinline__ void store16(float* p, bool vec, const float (&v)[4]) {
+    if (vec) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) p[i] = v[i];
+    }
+  }
   static __device__ __forceinline__ void open(const Raw& r, float (&v)[8]) {
     const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
@@ -112,6 +166,18 @@ template <> struct Elems<float> {
 template <class T, class T2> struct Elems16 {
   typedef uint4 Raw;
   static __device__ __forceinline__ Raw raw(const T* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ Raw from_lane(const Raw& r, int lane) { return kv8_from_lane(r, lane); }
+  static __device__ __forceinline__ Raw gather(const T* p) {           // not aligned
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      T2 h;
+      h.x = p[2 * i]; h.y = p[2 * i + 1];
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ void store16(T* p, bool vec, const float (&v)[8]) { Elems16::store(p, vec, v); }
   static __device__ __forceinline__ void open(const Raw& u, float (&v)[8]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -132,11 +198,7 @@ template <class T, class T2> struct Elems16 {
     if (vec) {
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        T2 h;
-        h.x = from(v[2 * i]); h.y = from(v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
+      for (int i = 0; i < 4; i++) w[i] = kv8_pack2<T>(v[2 * i], v[2 * i + 1]);
       *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll

@@ -60,37 +60,19 @@ __device__ __forceinline__ float km_exp2(float x) {
   return y;
 }
 
-// two f32 at a time
-__device__ __forceinline__ uint64_t km_two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void km_apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t km_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t km_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // 2^x of two numbers on the fused multiply-add pipe: x = n + r, |r| <= 1/2, a polynomial of degree 4 in r (minimax by Remez exchange, 2^-18.5)
 // and n into its exponent.  [-126, 127]; what is below is as good as 0, what is above is looked at again
 __device__ __forceinline__ void km_exp2_fma(float& a, float& b) {
   const float big = 12582912.f;                        // 1.5 * 2^23: the sum's last bits are the nearest whole number
-  const uint64_t x = km_two(fminf(fmaxf(a, -126.f), 127.f), fminf(fmaxf(b, -126.f), 127.f));
-  const uint64_t t = km_add2(x, km_two(big, big)), r = km_fma2(km_add2(t, km_two(-big, -big)), km_two(-1.f, -1.f), x);
-  uint64_t p = km_fma2(r, km_two(0.009570102207362652f, 0.009570102207362652f), km_two(0.05591785907745361f, 0.05591785907745361f));
-  p = km_fma2(p, r, km_two(0.240247443318367f, 0.240247443318367f));
-  p = km_fma2(p, r, km_two(0.6931217908859253f, 0.6931217908859253f));
-  p = km_fma2(p, r, km_two(0.9999992847442627f, 0.9999992847442627f));
+  const uint64_t x = kv8_two(fminf(fmaxf(a, -126.f), 127.f), fminf(fmaxf(b, -126.f), 127.f));
+  const uint64_t t = kv8_add2(x, kv8_two(big, big)), r = kv8_fma2(kv8_add2(t, kv8_two(-big, -big)), kv8_two(-1.f, -1.f), x);
+  uint64_t p = kv8_fma2(r, kv8_two(0.009570102207362652f, 0.009570102207362652f), kv8_two(0.05591785907745361f, 0.05591785907745361f));
+  p = kv8_fma2(p, r, kv8_two(0.240247443318367f, 0.240247443318367f));
+  p = kv8_fma2(p, r, kv8_two(0.6931217908859253f, 0.6931217908859253f));
+  p = kv8_fma2(p, r, kv8_two(0.9999992847442627f, 0.9999992847442627f));
   float pa, pb, ta, tb;
-  km_apart(p, pa, pb);
-  km_apart(t, ta, tb);
+  kv8_apart(p, pa, pb);
+  kv8_apart(t, ta, tb);
   a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
   b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
 }
@@ -385,11 +367,11 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
 #pragma unroll
         for (int h = 0; h < 4; h++) {
           const float4 sc = hd->sc[s][c + h];
-          const uint64_t f = km_two(f0 * sc.x, f0 * sc.x), b = km_two(sc.y - mm, sc.y - mm);
+          const uint64_t f = kv8_two(f0 * sc.x, f0 * sc.x), b = kv8_two(sc.y - mm, sc.y - mm);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             float x, y;
-            km_apart(km_fma2(km_two(__uint_as_float(w[h][i]), __uint_as_float(w[h][i + 1])), f, b), x, y);
+            kv8_apart(kv8_fma2(kv8_two(__uint_as_float(w[h][i]), __uint_as_float(w[h][i + 1])), f, b), x, y);
             w[h][i] = __float_as_uint(x); w[h][i + 1] = __float_as_uint(y);
           }
         }
@@ -409,10 +391,10 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
             if (!TWO && (i & 6) == 6) km_exp2_fma(u, v);       // a quarter of them beside the others (F32 keeps its two units' accuracy)
             else { u = km_exp2(u); v = km_exp2(v); }
             w[h][i] = __float_as_uint(u); w[h][i + 1] = __float_as_uint(v);
-            x[i >> 1 & 1] = km_add2(x[i >> 1 & 1], km_two(u, v));
+            x[i >> 1 & 1] = kv8_add2(x[i >> 1 & 1], kv8_two(u, v));
           }
           float y, z;
-          km_apart(km_add2(x[0], x[1]), y, z);
+          kv8_apart(kv8_add2(x[0], x[1]), y, z);
           part[h] = y + z;
         }
         const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));

@@ -3,8 +3,9 @@
 //   code = e4m3(x / scale), nearest even, +-448 beyond
 // When a block already holds older tokens its scale only grows: E = max(E of the new values, E so far), and the older codes are
 // rounded to e4m3 again after division by the power of two (exact but for what falls below the format's normal range, 2^-6).
-// Both kernels move each byte once and are bound by memory: one block of threads per (cache block, head, keys or values), which holds
-// all its new values in registers between the maximum and the rounding.
+// Both kernels move each byte once and are bound by memory, or for few tokens by the chain of look-ups: the sequence of a work item,
+// its lengths, its block.  A group of threads does that once and goes over several (head, keys or values) units of the block: it holds a
+// unit's new values in registers between the maximum and the rounding, and the next unit's are on the way meanwhile.
 #include <algorithm>
 #include "kv8.cuh"
 
@@ -47,125 +48,205 @@ struct Kv8RowsParams {
   void *k, *v;                    // rows (read by the writing kernel, written by the reading one)
   int64_t k_stride, v_stride;     // elements
   int k_vec, v_vec;
+  int each;                       // items of a sequence, 0: as kv8_item finds them
   int* status;
 };
 
-constexpr int kKv8Threads = 256, kKv8Most = 128 * 128 / 8 / kKv8Threads;     // pieces of eight values a thread holds at most
+constexpr int kKv8Threads = 256;
 
-template <class T, int D>
+// THREADS threads a work item (32 or 256), each with up to MOST pieces of eight values of a unit
+template <class T, int D, int THREADS, int MOST>
 __global__ void __launch_bounds__(kKv8Threads) kv8_write_kernel(const Kv8RowsParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float s_max[kKv8Threads / 32];
-  const int tid = threadIdx.x, h = blockIdx.y, sh = p.c.shift;
-  const bool values = blockIdx.z;
-  int id;
-  const Kv8Item it = kv8_item(p.b, p.c, blockIdx.x, p.status, id);
-  if (it.n == 0 || id < 0) return;
-  const size_t head = (size_t)id * p.c.heads + h;
-  uint8_t* codes = (values ? p.c.v : p.c.k) + ((head << sh) * D);
-  float* scale = (values ? p.c.vs : p.c.ks) + head;
-  const int64_t stride = values ? p.v_stride : p.k_stride;
-  const bool vec = values ? p.v_vec : p.k_vec;
-  const T* rows = static_cast<const T*>(values ? p.v : p.k) + it.row * stride + (int64_t)h * D;
-  const float was = it.at ? *scale : 0.f;
-  const int pieces = it.n * (D / 8);
-
-  float v[kKv8Most][8];
-  float top = 0.f;
-  bool nan = false;
+  constexpr int kGroups = kKv8Threads / THREADS, kRow = D / 8, kWarps = THREADS / 32;
+  __shared__ float s_max[2][kWarps];
+  const int tid = threadIdx.x % THREADS, sh = p.c.shift, units = 2 * p.c.heads, step = gridDim.y * kGroups;
+  int s;
+  const Kv8Item it = kv8_item(p.b, sh, p.each, blockIdx.x, p.status, s);
+  if (it.n == 0) return;
+  const int pieces = it.n * kRow;
+  typename Elems<T>::Raw r[MOST], next[MOST];
+  auto load = [&](int u) {        // unit u: head u / 2, its keys or its values
+    const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
+    const int64_t stride = values ? p.v_stride : p.k_stride;
+    const T* rows = static_cast<const T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
+    if (vec) {
 #pragma unroll
-  for (int i = 0; i < kKv8Most; i++) {
-    const int c = tid + i * kKv8Threads;
-    if (c < pieces) Elems<T>::load(rows + (c / (D / 8)) * stride + c % (D / 8) * 8, vec, v[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < kKv8Most; i++) {
-    if (tid + i * kKv8Threads < pieces)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        if (v[i][j] != v[i][j]) { nan = true; v[i][j] = 0.f; }      // the cache holds no NaN: its attention multiplies masked rows by 0
-        const float a = fabsf(v[i][j]);
-        if (a <= 3.402823466e38f) top = fmaxf(top, a);              // an infinity becomes the largest code
+      for (int i = 0; i < MOST; i++) {
+        const int c = tid + i * THREADS;
+        if (c < pieces) next[i] = Elems<T>::raw(rows + (c / kRow) * stride + c % kRow * 8);
       }
-  }
-  if (nan) atomicCAS(p.status, 0, kDevNan);
-  top = warp_max(top);
-  if ((tid & 31) == 0) s_max[tid >> 5] = top;
-  __syncthreads();
+    } else {
 #pragma unroll
-  for (int i = 0; i < kKv8Threads / 32; i++) top = fmaxf(top, s_max[i]);
-  // top = 1.m * 2^e <= 448 * 2^E = 1.75 * 2^(8 + E)
-  const uint32_t u = __float_as_uint(top);
-  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  e = min(max(e, kKv8MinExp), kKv8MaxExp);
-  int e_old = e;
-  if (it.at) { e_old = kv8_exp(was); e = max(e, e_old); }
-  const float inv = kv8_pow2(-e);
-#pragma unroll
-  for (int i = 0; i < kKv8Most; i++) {
-    const int c = tid + i * kKv8Threads;
-    if (c < pieces)
-      *reinterpret_cast<uint2*>(codes + (it.at + c / (D / 8)) * D + c % (D / 8) * 8) =
-          make_uint2(kv8_codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                     kv8_codes4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
-  }
-  if (e > e_old) {                                                  // older tokens of the block move to the larger scale
-    const float f = kv8_pow2(e_old - e);
-    for (int c = tid; c < it.at * (D / 16); c += kKv8Threads) {
-      uint4* q = reinterpret_cast<uint4*>(codes) + c;
-      uint32_t w[4] = {q->x, q->y, q->z, q->w};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float2 a = kv8_float2(w[j]), b = kv8_float2(w[j] >> 16);
-        w[j] = kv8_codes4(a.x * f, a.y * f, b.x * f, b.y * f);
+      for (int i = 0; i < MOST; i++) {
+        const int c = tid + i * THREADS;
+        if (c < pieces) next[i] = Elems<T>::gather(rows + (c / kRow) * stride + c % kRow * 8);
       }
-      *q = make_uint4(w[0], w[1], w[2], w[3]);
     }
+  };
+  int u = blockIdx.y * kGroups + threadIdx.x / THREADS;
+  if (u < units) load(u);
+  const int id = kv8_block(p.b, p.c.n_blocks, s, it, p.status);
+  if (id < 0) return;
+  float was = 0.f;
+  if (it.at && u < units) was = ((u & 1) ? p.c.vs : p.c.ks)[(size_t)id * p.c.heads + (u >> 1)];
+  for (int turn = 0; u < units; u += step, turn ^= 1) {
+    const size_t head = (size_t)id * p.c.heads + (u >> 1);
+    uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D;
+    float* scale = ((u & 1) ? p.c.vs : p.c.ks) + head;
+    const float old = was;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) r[i] = next[i];
+    if (u + step < units) {
+      load(u + step);
+      if (it.at) was = (((u + step) & 1) ? p.c.vs : p.c.ks)[(size_t)id * p.c.heads + ((u + step) >> 1)];
+    }
+    float top = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < MOST; i++)
+      if (tid + i * THREADS < pieces) {
+        float v[8];
+        Elems<T>::open(r[i], v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float a = fabsf(v[j]);
+          nan |= a != a;
+          if (a <= 3.402823466e38f) top = fmaxf(top, a);            // an infinity becomes the largest code
+        }
+      }
+    top = warp_max(top);
+    if (THREADS > 32) {
+      if ((tid & 31) == 0) s_max[turn][tid >> 5] = top;
+      __syncthreads();                                              // (also: every thread has read the scale that is written below)
+#pragma unroll
+      for (int i = 0; i < kWarps; i++) top = fmaxf(top, s_max[turn][i]);
+    }
+    // top = 1.m * 2^e <= 448 * 2^E = 1.75 * 2^(8 + E)
+    const uint32_t bits = __float_as_uint(top);
+    int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    e = min(max(e, kKv8MinExp), kKv8MaxExp);
+    int e_old = e;
+    if (it.at) { e_old = kv8_exp(old); e = max(e, e_old); }
+    const float inv = kv8_pow2(-e);
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int c = tid + i * THREADS;
+      if (c < pieces) {
+        float v[8];
+        Elems<T>::open(r[i], v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] *= inv;
+        if (nan) {                                                  // the cache holds none: its attention multiplies masked rows by 0
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = v[j] != v[j] ? 0.f : v[j];
+        }
+        *reinterpret_cast<uint2*>(codes + (it.at + c / kRow) * D + c % kRow * 8) =
+            make_uint2(kv8_codes4(v[0], v[1], v[2], v[3]), kv8_codes4(v[4], v[5], v[6], v[7]));
+      }
+    }
+    if (nan) atomicCAS(p.status, 0, kDevNan);
+    if (e > e_old) {                                                // older tokens of the block move to the larger scale
+      const float f = kv8_pow2(e_old - e);
+#pragma unroll 4
+      for (int c = tid; c < it.at * (D / 16); c += THREADS) {
+        uint4* q = reinterpret_cast<uint4*>(codes) + c;
+        uint32_t w[4] = {q->x, q->y, q->z, q->w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 a = kv8_float2(w[j]), b = kv8_float2(w[j] >> 16);
+          w[j] = kv8_codes4(a.x * f, a.y * f, b.x * f, b.y * f);
+        }
+        *q = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (THREADS == 32) __syncwarp();
+    if (tid == 0) *scale = kv8_pow2(e);
   }
-  if (tid == 0) *scale = kv8_pow2(e);                               // every thread read it before the barrier above
 }
 
-template <class T, int D>
+// 16 bytes of a row a thread and step: eight values, four of F32; up to MOST steps a unit
+template <class T, int D, int MOST>
 __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8RowsParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int h = blockIdx.y, sh = p.c.shift;
-  const bool values = blockIdx.z;
-  int id;
-  const Kv8Item it = kv8_item(p.b, p.c, blockIdx.x, p.status, id);
+  constexpr int V = 16 / sizeof(T), kRow = D / V;
+  const int sh = p.c.shift, units = 2 * p.c.heads;
+  int s;
+  const Kv8Item it = kv8_item(p.b, sh, p.each, blockIdx.x, p.status, s);
   if (it.n == 0) return;
-  const size_t head = (size_t)max(id, 0) * p.c.heads + h;
-  const uint8_t* codes = (values ? p.c.v : p.c.k) + (head << sh) * D + it.at * D;
-  const float scale = id < 0 ? 0.f : (values ? p.c.vs : p.c.ks)[head];
-  const int64_t stride = values ? p.v_stride : p.k_stride;
-  const bool vec = values ? p.v_vec : p.k_vec;
-  T* rows = static_cast<T*>(values ? p.v : p.k) + it.row * stride + (int64_t)h * D;
-  for (int c = threadIdx.x; c < it.n * (D / 16); c += kKv8Threads) {
-    uint4 q = make_uint4(0, 0, 0, 0);
-    if (id >= 0) q = reinterpret_cast<const uint4*>(codes)[c];
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    T* dst = rows + (c / (D / 16)) * stride + c % (D / 16) * 16;
+  const int id = kv8_block(p.b, p.c.n_blocks, s, it, p.status), pieces = it.n * kRow;
+  uint32_t w[MOST][V / 4], next[MOST][V / 4] = {};
+  float scale = 0.f, next_scale = 0.f;
+  auto load = [&](int u) {
+    if (id < 0) return;
+    const size_t head = (size_t)id * p.c.heads + (u >> 1);
+    const uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D + it.at * D;
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-      float o[8];
+    for (int i = 0; i < MOST; i++) {
+      const int c = threadIdx.x + i * kKv8Threads;
+      if (c < pieces) {
+        if (V == 8) {
+          const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes) + c);
+          next[i][0] = q.x; next[i][V / 4 - 1] = q.y;
+        } else {
+          next[i][0] = __ldg(reinterpret_cast<const uint32_t*>(codes) + c);
+        }
+      }
+    }
+    next_scale = __ldg(((u & 1) ? p.c.vs : p.c.ks) + head);
+  };
+  int u = blockIdx.y;
+  if (u < units) load(u);
+  for (; u < units; u += gridDim.y) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float2 a = kv8_float2(w[2 * half + (j >> 1)] >> (16 * (j & 1)));
+    for (int i = 0; i < MOST; i++)
+#pragma unroll
+      for (int j = 0; j < V / 4; j++) w[i][j] = next[i][j];
+    scale = next_scale;
+    if (u + gridDim.y < units) load(u + gridDim.y);
+    const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
+    const int64_t stride = values ? p.v_stride : p.k_stride;
+    T* rows = static_cast<T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int c = threadIdx.x + i * kKv8Threads;
+      if (c >= pieces) break;
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V / 2; j++) {
+        const float2 a = kv8_float2(w[i][j >> 1] >> (16 * (j & 1)));
         o[2 * j] = a.x * scale; o[2 * j + 1] = a.y * scale;
       }
-      Elems<T>::store(dst + 8 * half, vec, o);
+      Elems<T>::store16(rows + (c / kRow) * stride + c % kRow * V, vec, o);
     }
   }
 }
 
-template <bool WRITE, class T>
-static int launch_rows(const Kv8RowsParams& p, int D, cudaStream_t st) {
-  const dim3 grid((unsigned)kv8_items(p.b.n_tokens, p.b.n_seq, p.c.shift), p.c.heads, 2);
+template <class T, int D>
+static int launch_rows(bool write, Kv8RowsParams& p, cudaStream_t st) {
+  const int sh = p.c.shift, units = 2 * p.c.heads;
+  // items: every sequence's most, or as its rows have it
+  const int64_t each = kv8_touched(p.b.max_new, sh), all = kv8_items(p.b.n_tokens, p.b.n_seq, sh);
+  const int64_t items = std::min(each * p.b.n_seq, all);
+  p.each = each * p.b.n_seq <= all ? (int)each : 0;
+  // a warp a unit while its new rows are few; for more a block, which goes over the units of a block while there are blocks enough
+  // (reading 16 sequences of up to 8192 tokens: 90.5 us with 4 or 8 blocks an SM, 84.7 with 16, 82.7 with 32, 87.3 with 64)
+  if (items > 0x7fffffff) return fail(kErrLimit, "kv8: too many rows");
+  const bool few = (int64_t)std::min(p.b.max_new, 1 << sh) * (D / 8) <= 64;
+  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(units, items * units / (148 * (write ? 8 : 32))));
+  const dim3 grid((unsigned)items, write && few ? (units + 7) / 8 : (units + per - 1) / per);
   auto go = [&](auto kern) { return launch_pdl(kern, grid, dim3(kKv8Threads), 0, st, p); };
-  if (WRITE) MSB_CUDA(D == 64 ? go(kv8_write_kernel<T, 64>) : go(kv8_write_kernel<T, 128>));
-  else MSB_CUDA(D == 64 ? go(kv8_read_kernel<T, 64>) : go(kv8_read_kernel<T, 128>));
-  MSB_LAUNCH_CHECK(WRITE ? "kv8_write" : "kv8_read");
+  if (!write) {
+    const int pieces = (D * (int)sizeof(T) / 16) << sh;
+    MSB_CUDA(pieces <= 4 * kKv8Threads ? go(kv8_read_kernel<T, D, 4>) : pieces <= 8 * kKv8Threads ? go(kv8_read_kernel<T, D, 8>)
+                                                                                                   : go(kv8_read_kernel<T, D, 16>));
+  }
+  else if (few) MSB_CUDA(go(kv8_write_kernel<T, D, 32, 2>));
+  else if ((D / 8) << sh <= 4 * kKv8Threads) MSB_CUDA(go(kv8_write_kernel<T, D, 256, 4>));
+  else MSB_CUDA(go(kv8_write_kernel<T, D, 256, 8>));
+  MSB_LAUNCH_CHECK(write ? "kv8_write" : "kv8_read");
   return kOk;
 }
 
@@ -181,12 +262,11 @@ static int kv8_rows(bool write, const msb_kv8_cache* c, const msb_kv8_batch* b, 
   Tables tb;
   if ((rc = get_tables(&tb))) return rc;
   p.k = k; p.v = v; p.k_stride = k_stride; p.v_stride = v_stride; p.k_vec = kvec; p.v_vec = vvec; p.status = tb.status;
-  const int D = c->head_dim;
-  if (write)
-    return elem_type == F32 ? launch_rows<true, float>(p, D, st) : elem_type == F16 ? launch_rows<true, __half>(p, D, st)
-                                                                                    : launch_rows<true, __nv_bfloat16>(p, D, st);
-  return elem_type == F32 ? launch_rows<false, float>(p, D, st) : elem_type == F16 ? launch_rows<false, __half>(p, D, st)
-                                                                                   : launch_rows<false, __nv_bfloat16>(p, D, st);
+#define KV8_GO(T) return c->head_dim == 64 ? launch_rows<T, 64>(write, p, st) : launch_rows<T, 128>(write, p, st)
+  if (elem_type == F32) KV8_GO(float);
+  if (elem_type == F16) KV8_GO(__half);
+  KV8_GO(__nv_bfloat16);
+#undef KV8_GO
 }
 int kv8_write(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, const void* k, const void* v, int64_t k_stride,
               int64_t v_stride, cudaStream_t st) {

@@ -28,6 +28,9 @@ KV8_HD bool kv8_seq_of(int r0, int r1, int len, int n_tokens, int max_new, int m
 KV8_HD int kv8_first_item(int start, int s, int shift) { return (start >> shift) + 2 * s; }
 inline int64_t kv8_items(int n_tokens, int n_seq, int shift) { return (int64_t)(n_tokens >> shift) + 2 * (int64_t)n_seq; }
 
+// blocks that `n` new tokens lie in, at most
+inline int kv8_touched(int n, int shift) { return (int)(((int64_t)n + (2 << shift) - 2) >> shift); }
+
 // The j-th item of a sequence: its block's place in the table, first row, first token inside the block, tokens (0: nothing to do).
 struct Kv8Item { int blk, row, at, n; };
 KV8_HD Kv8Item kv8_item_of(const Kv8Seq& q, int j, int shift) {

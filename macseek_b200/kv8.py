@@ -16,21 +16,15 @@ def _want(ok, what):
         raise _lib.MsbError(what)
 
 
-def _on_stream(e, device):
-    """The library works on the current device: it has to be the stream's and the tensors'."""
-    _want(e.stream.device == device, "tensors on %s, the stream on %s" % (device, e.stream.device))
-    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else _NO_GUARD
-
-
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *a):
-        return False
-
-
-_NO_GUARD = _NoGuard()
+def _call(e, device, fn, *args):
+    """fn(*args) with `device` current (the library works on the current device), which has to be the stream's too."""
+    st = e.stream
+    if st.device_index != device.index:
+        raise _lib.MsbError("tensors on %s, the stream on %s" % (device, st.device))
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, st.cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, st.cuda_stream)
 
 
 class Cache:
@@ -59,7 +53,7 @@ class Cache:
         self.n_blocks, self.kv_heads, self.block, self.head_dim = k.shape
         self.c = _lib.Kv8CacheC(self.n_blocks, self.kv_heads, self.head_dim, self.block, k.data_ptr(), v.data_ptr(),
                                 k_scale.data_ptr(), v_scale.data_ptr())
-        self.ref = C.byref(self.c)
+        self.ref, self.addr = C.byref(self.c), C.addressof(self.c)
 
 
 class Batch:
@@ -77,7 +71,7 @@ class Batch:
         self.n_seq, self.n_tokens, self.max_new, self.max_len = n, n_tokens, max_new, max_len
         self.c = _lib.Kv8BatchC(n, n_tokens, max_new, max_len, seq_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
                                 table.shape[1])
-        self.ref = C.byref(self.c)
+        self.ref, self.addr = C.byref(self.c), C.addressof(self.c)
 
 
 def _rows(name, t, n_tokens, heads, dim, device):
@@ -94,23 +88,28 @@ def _stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
-def _kv(e, cache, batch, k, v, call):
+_WRITE, _READ, _ATTN = (_lib.address(f) for f in (_lib.lib.msb_kv8_write, _lib.lib.msb_kv8_read, _lib.lib.msb_kv8_attn))
+
+
+def _kv(e, cache, batch, k, v, call, what):
     dev = cache.device
-    _want(batch.device == dev, "kv8: cache and batch on different devices")
-    ty = _rows("k", k, batch.n_tokens, cache.kv_heads, cache.head_dim, dev)
-    _want(_rows("v", v, batch.n_tokens, cache.kv_heads, cache.head_dim, dev) == ty, "k and v must be of one type")
-    with _on_stream(e, dev):
-        _lib.check(call(cache.ref, batch.ref, ty, k.data_ptr(), v.data_ptr(), _stride(k), _stride(v), e.handle))
+    rc = _call(e, dev, _lib.host().msb_host_kv8_rows, k, v, cache.addr, batch.addr, dev.index, call) if batch.device == dev else 1
+    if rc > 0:                     # not plainly right: say why
+        _want(batch.device == dev, "%s: cache and batch on different devices" % what)
+        ty = _rows("k", k, batch.n_tokens, cache.kv_heads, cache.head_dim, dev)
+        _want(_rows("v", v, batch.n_tokens, cache.kv_heads, cache.head_dim, dev) == ty, "k and v must be of one type")
+        _want(False, "%s: k and v must be rows of the batch and the cache" % what)
+    _lib.check(rc)
 
 
 def encode_kv8_write(e: Enc, cache: Cache, batch: Batch, k, v):
     """New rows k, v [n_tokens][kv_heads][head_dim] into the cache."""
-    _kv(e, cache, batch, k, v, _lib.lib.msb_kv8_write)
+    _kv(e, cache, batch, k, v, _WRITE, "kv8_write")
 
 
 def encode_kv8_read(e: Enc, cache: Cache, batch: Batch, k, v):
     """The batch's rows of the cache into k, v."""
-    _kv(e, cache, batch, k, v, _lib.lib.msb_kv8_read)
+    _kv(e, cache, batch, k, v, _READ, "kv8_read")
 
 
 def attn_scratch(cache: Cache, batch: Batch, heads):
@@ -125,15 +124,12 @@ def encode_kv8_attn(e: Enc, cache: Cache, batch: Batch, q, out, scratch, scale=N
     """Attention of the rows q [n_tokens][heads][head_dim] over the cache, which holds their tokens already, into out
     (scale: head_dim^-0.5 if None; window 0: everything up to the row's own token; sinks: F32 [heads] or None)."""
     dev = cache.device
-    heads = q.shape[1]
-    ty = _rows("q", q, batch.n_tokens, heads, cache.head_dim, dev)
-    _want(_rows("out", out, batch.n_tokens, heads, cache.head_dim, dev) == ty, "q and out must be of one type")
-    _want(batch.device == dev and scratch.device == dev, "kv8: cache, batch and scratch on different devices")
-    if sinks is not None:
-        _want(sinks.device == dev and sinks.dtype == torch.float32 and tuple(sinks.shape) == (heads,) and sinks.is_contiguous(),
-              "sinks must be contiguous float32 [%d]" % heads)
-    with _on_stream(e, dev):
-        _lib.check(_lib.lib.msb_kv8_attn(cache.ref, batch.ref, ty, q.data_ptr(), _stride(q), heads,
-                                         cache.head_dim ** -0.5 if scale is None else scale, window,
-                                         None if sinks is None else sinks.data_ptr(), out.data_ptr(), _stride(out),
-                                         scratch.data_ptr(), scratch.numel() * scratch.element_size(), e.handle))
+    rc = _call(e, dev, _lib.host().msb_host_kv8_attn, q, out, scratch, sinks, cache.addr, batch.addr, dev.index,
+               cache.head_dim ** -0.5 if scale is None else scale, window, _ATTN) if batch.device == dev else 1
+    if rc > 0:                     # not plainly right: say why
+        _want(batch.device == dev and scratch.device == dev, "kv8_attn: cache, batch and scratch on different devices")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        ty = _rows("q", q, batch.n_tokens, heads, cache.head_dim, dev)
+        _want(_rows("out", out, batch.n_tokens, heads, cache.head_dim, dev) == ty, "q and out must be of one type")
+        _want(False, "kv8_attn: sinks must be contiguous float32 [%d] or None" % heads)
+    _lib.check(rc)

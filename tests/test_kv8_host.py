@@ -11,6 +11,7 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 
 PROGRAM = r"""
 #include "kv8_index.h"
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -54,6 +55,20 @@ int main() {
       NEED(it.row >= 0 && it.row + it.n <= n_tokens);
       NEED(it.blk * block + it.at == q.len - q.n + it.row - q.row);
       for (int r = 0; r < it.n; r++) seen[it.row + r]++;
+    }
+    if (!broken)
+      for (int r = 0; r < n_tokens; r++) NEED(seen[r] == (r < start[n_seq]));
+    // the other numbering: as many items for every sequence as the longest needs
+    const int each = kv8_touched(max_new, shift);
+    std::fill(seen.begin(), seen.end(), 0);
+    for (int s = 0; s < n_seq; s++) {
+      Kv8Seq q;
+      kv8_seq_of(start[s], start[s + 1], len[s], n_tokens, max_new, max_len, q);
+      for (int j = 0; j < each; j++) {
+        const Kv8Item it = kv8_item_of(q, j, shift);
+        NEED(it.n == 0 || (it.blk < stride && it.at + it.n <= block && it.row + it.n <= n_tokens && it.n <= max_new));
+        for (int r = 0; r < it.n; r++) seen[it.row + r]++;
+      }
     }
     if (!broken)
       for (int r = 0; r < n_tokens; r++) NEED(seen[r] == (r < start[n_seq]));
@@ -168,13 +183,14 @@ def test_mirror_refuses_tensors_of_the_host():
 
 class _Stream:
     device = torch.device("cuda", 1)
+    device_index = 1
 
 
 def test_mirror_refuses_another_device_than_the_streams():
     from macseek_b200 import _lib, kv8
     e = type("E", (), {"stream": _Stream()})()
     with pytest.raises(_lib.MsbError, match="stream"):
-        kv8._on_stream(e, torch.device("cuda", 0))
+        kv8._call(e, torch.device("cuda", 0), None)
 
 
 @pytest.mark.parametrize("shape,stride,ok", [((3, 2, 64), (128, 64, 1), True), ((3, 2, 64), (400, 64, 1), True), ((1, 2, 64), (9, 64, 1), True),
