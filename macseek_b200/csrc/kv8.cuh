@@ -131,6 +131,9 @@ template <> struct Elems<float> {
     for (int i = 0; i < 8; i++) w[i] = __float_as_uint(p[i]);
     return Raw{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
   }
+  static __device__ __forceinline__ uint4 pack16(const float (&v)[8], int k) {     // 16 bytes of eight elements' 32
+    return make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3]));
+  }
   static __device__ __forceinline__ void store16(float* p, bool vec, const float (&v)[4]) {
     if (vec) {
       *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -176,6 +179,9 @@ template <class T, class T2> struct Elems16 {
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint4 pack16(const float (&v)[8], int) {
+    return make_uint4(kv8_pack2<T>(v[0], v[1]), kv8_pack2<T>(v[2], v[3]), kv8_pack2<T>(v[4], v[5]), kv8_pack2<T>(v[6], v[7]));
   }
   static __device__ __forceinline__ void store16(T* p, bool vec, const float (&v)[8]) { Elems16::store(p, vec, v); }
   static __device__ __forceinline__ void open(const Raw& u, float (&v)[8]) {

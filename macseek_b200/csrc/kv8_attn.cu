@@ -13,7 +13,7 @@
 
 namespace msb {
 
-constexpr int kKdWarps = 4, kKdStages = 2, kKdStep = 32, kKdRows = 16, kKmStep = 128;
+constexpr int kKdWarps = 4, kKdStages = 2, kKdStep = kKv8FewStep, kKdRows = kKv8FewRows;
 
 __device__ __forceinline__ void kd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -339,30 +339,36 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   }
 }
 
-// The splits of one row joined, in their order; one block per (token, query head), a warp takes every fourth split.
-template <class T, int D>
+// The splits of one row joined, in their order: WARPS warps a (token, query head), each every WARPS-th split.
+template <class T, int D, int WARPS>
 __global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnParams p) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int V = D / 32, kRows = 4 / WARPS;
   __shared__ float s_m[4], s_l[4];
   __shared__ __align__(16) float s_o[4][D];
-  constexpr int V = D / 32;
-  const int head = blockIdx.y, tok = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int s = kv8_find(p.b.n_seq, tok, [&](int i) { return __ldg(p.b.seq_start + i); });
-  const Kv8Seq sq = kv8_seq(p.b, s, p.status);
-  const int i = tok - sq.row;
-  if (i < 0 || i >= sq.n) return;
-  const int row = i * p.G + head % p.G, m0 = row / p.tile * p.tile, m1 = min(m0 + p.tile, sq.n * p.G);
-  const Kv8Range kr = kv8_range(sq, m0, m1, p.G, p.window, p.step);
-  const int n = (kr.hi - kr.lo + p.chunk - 1) / p.chunk;
-  const size_t stride = (size_t)p.b.n_tokens * p.heads, at = (size_t)tok * p.heads + head;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WARPS;
+  const int64_t at = (int64_t)blockIdx.x * kRows + warp / WARPS;        // row of the rows' products: token * heads + head
+  const int tok = (int)(at / p.heads), head = (int)(at - (int64_t)tok * p.heads);
+  int n = 0;
+  if (tok < p.b.n_tokens) {
+    const int s = kv8_find(p.b.n_seq, tok, [&](int i) { return __ldg(p.b.seq_start + i); });
+    const Kv8Seq sq = kv8_seq(p.b, s, p.status);
+    const int i = tok - sq.row;
+    if (i >= 0 && i < sq.n) {
+      const int row = i * p.G + head % p.G, m0 = row / p.tile * p.tile, m1 = min(m0 + p.tile, sq.n * p.G);
+      const Kv8Range kr = kv8_range(sq, m0, m1, p.G, p.window, p.step);
+      n = (kr.hi - kr.lo + p.chunk - 1) / p.chunk;
+    }
+  }
+  const size_t stride = (size_t)p.b.n_tokens * p.heads;
   const float2* ml = reinterpret_cast<const float2*>(kv8_part_ml(p, D)) + at;
   const float* po = p.part + at * D + lane * V;
   float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
   for (int j = 0; j < V; j++) o[j] = 0.f;
 #pragma unroll 4
-  for (int x = warp; x < n; x += 4) {
+  for (int x = part; x < n; x += WARPS) {
     const float2 a = __ldcg(ml + x * stride);
     float v[V];
 #pragma unroll
@@ -379,17 +385,20 @@ __global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnParams 
   if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
 #pragma unroll
   for (int j = 0; j < V; j += 2) *reinterpret_cast<float2*>(&s_o[warp][lane * V + j]) = make_float2(o[j], o[j + 1]);
-  __syncthreads();
-  if (threadIdx.x >= D / 8) return;
-  const int d = threadIdx.x * 8;
-  const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  if (WARPS == 1) __syncwarp();
+  else __syncthreads();
+  if (n == 0 || part || lane >= D / 8) return;
+  const int d = lane * 8;
+  float M = s_m[warp];
+#pragma unroll
+  for (int w = 1; w < WARPS; w++) M = fmaxf(M, s_m[warp + w]);
   float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const float f = s_m[w] == -INFINITY ? 0.f : kd_exp2(s_m[w] - M);
-    sum += s_l[w] * f;
+  for (int w = 0; w < WARPS; w++) {
+    const float f = s_m[warp + w] == -INFINITY ? 0.f : kd_exp2(s_m[warp + w] - M);
+    sum += s_l[warp + w] * f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] += s_o[w][d + j] * f;
+    for (int j = 0; j < 8; j++) v[j] += s_o[warp + w][d + j] * f;
   }
   if (p.sinks) sum += kd_exp2(p.sinks[head] * kLog2e - (M == -INFINITY ? 0.f : M));
   const float inv = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
@@ -399,22 +408,6 @@ __global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnParams 
 }
 
 // ---------------------------------------------------------------- host side
-struct Kv8Plan { int many, tiles, chunk, splits, most; };      // most: splits at most, for any window
-static Kv8Plan kv8_plan(const Kv8Batch& b, int kv_heads, int heads, int window, int elem_type, int sms) {
-  const int G = heads / kv_heads;
-  Kv8Plan pl;
-  pl.many = (int64_t)b.max_new * G > 32;
-  const int rows = pl.many ? kv8_many_rows(elem_type) : kKdRows, step = pl.many ? kKmStep : kKdStep;
-  pl.tiles = (int)(((int64_t)b.max_new * G + rows - 1) / rows);
-  const int64_t units = (int64_t)pl.tiles * kv_heads * b.n_seq;
-  // few rows: three blocks an SM, and six times as many for sequences whose lengths differ
-  const int64_t want = pl.many ? 2 * sms : (int64_t)3 * sms * (b.n_seq > 1 ? 6 : 1);
-  const int least = pl.many ? 512 : 128;
-  const Kv8Split sp = kv8_split(kv8_span(b.max_len, rows, G, window, step), units, want, least, pl.many ? kKmStep : 64);
-  pl.chunk = sp.chunk; pl.splits = sp.splits;
-  pl.most = kv8_most_splits(b.max_len, units, want, least);
-  return pl;
-}
 static int kv8_sms(int* sms) {
   int dev = 0;
   MSB_CUDA(cudaGetDevice(&dev));
@@ -432,7 +425,12 @@ size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, in
   Kv8Cache cc; Kv8Batch bb;
   int sms;
   if (kv8_check(c, b, "kv8_attn_scratch_bytes", &cc, &bb) || kv8_heads_check(c, heads, "kv8_attn_scratch_bytes") || kv8_sms(&sms)) return 0;
-  const int most = std::max(kv8_plan(bb, cc.heads, heads, 0, F32, sms).most, kv8_plan(bb, cc.heads, heads, 0, BF16, sms).most);
+  // (a window may change which kernel runs, and a split that is none needs no room)
+  int most = 1;
+  for (int f32 = 0; f32 < 2; f32++) {
+    const Kv8Most m = kv8_most(bb.n_seq, bb.max_new, bb.max_len, cc.heads, heads, f32, sms);
+    most = std::max(most, std::max(m.few, m.many));
+  }
   return 16 + kv8_part_bytes(bb, heads, c->head_dim, most);
 }
 
@@ -453,7 +451,11 @@ static int launch_attn(const Kv8AttnParams& p, const Kv8Plan& pl, int elem_type,
     MSB_LAUNCH_CHECK("kv8_attn");
   }
   if (pl.splits > 1) {
-    MSB_CUDA(launch_pdl(kv8_attn_join_kernel<T, D>, dim3(p.b.n_tokens, p.heads), dim3(128), 0, st, p));
+    // a warp a row for few parts or many rows, four where a row's parts would be a long chain
+    const int64_t rows = (int64_t)p.b.n_tokens * p.heads;
+    const bool alone = pl.splits <= 8 || rows >= 32768;
+    MSB_CUDA(launch_pdl(alone ? kv8_attn_join_kernel<T, D, 1> : kv8_attn_join_kernel<T, D, 4>, dim3((unsigned)(alone ? (rows + 3) / 4 : rows)),
+                        dim3(128), 0, st, p));
     MSB_LAUNCH_CHECK("kv8_attn_join");
   }
   return kOk;
@@ -473,8 +475,9 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   int dev, sms;
   MSB_CUDA(cudaGetDevice(&dev));
   if ((rc = kv8_sms(&sms))) return rc;
-  const Kv8Plan pl = kv8_plan(p.b, p.c.heads, heads, window, elem_type, sms);
+  const Kv8Plan pl = kv8_plan(p.b.n_seq, p.b.max_new, p.b.max_len, p.c.heads, heads, c->head_dim, elem_type == F32, window, sms);
   if (pl.many ? pl.tiles > 65535 : (int64_t)p.c.heads * pl.tiles > 65535) return fail(kErrLimit, "%s: too many rows", what);
+  if ((int64_t)p.b.n_tokens * heads > 0x7fffffff) return fail(kErrLimit, "%s: too many rows", what);
   const size_t need = kv8_part_bytes(p.b, heads, c->head_dim, pl.splits);
   if (need && (!scratch || scratch_bytes < need)) return fail(kErrScratch, "%s: scratch too small (%zu < %zu)", what, scratch_bytes, need);
   if (need && (reinterpret_cast<uintptr_t>(scratch) & 15)) return fail(kErrArg, "%s: scratch must be 16-byte aligned", what);
@@ -482,7 +485,7 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   if ((rc = get_tables(&tb))) return rc;
   p.q = q; p.out = out; p.q_stride = q_stride; p.out_stride = out_stride; p.sinks = sinks; p.part = static_cast<float*>(scratch);
   p.scale = scale; p.heads = heads; p.G = heads / p.c.heads; p.window = window; p.chunk = pl.chunk; p.splits = pl.splits;
-  p.tile = pl.many ? kv8_many_rows(elem_type) : kKdRows; p.step = pl.many ? kKmStep : kKdStep;
+  p.tile = pl.rows; p.step = pl.step;
   p.q_vec = qv; p.out_vec = ov; p.status = tb.status;
 #define KV8_GO(T) return c->head_dim == 64 ? launch_attn<T, 64>(p, pl, elem_type, st, dev) : launch_attn<T, 128>(p, pl, elem_type, st, dev)
   if (elem_type == F32) KV8_GO(float);

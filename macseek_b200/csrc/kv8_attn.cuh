@@ -26,7 +26,7 @@ struct Kv8AttnParams {
   int* status;
 };
 
-int kv8_many_rows(int elem_type);      // rows of a block of the kernel for many rows, and its launch over `groups` blocks of rows
+// the kernel for many rows over `groups` blocks of rows
 int kv8_attn_many(const Kv8AttnParams& p, int groups, int elem_type, int D, cudaStream_t st, int dev);
 
 #ifdef __CUDACC__

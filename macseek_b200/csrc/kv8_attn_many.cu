@@ -1,40 +1,43 @@
 // Attention over the 8-bit cache (kv8_attn.cuh) for many query rows: chunks of prompts, whole prompts, large groups.
 //
-// Two products a tile of 128 keys, both on tcgen05 with halves and fp32 sums: S = Q K^T, operands in shared memory, and O += P V, the
+// Two products a tile of 64 keys, both on tcgen05 with halves and fp32 sums: S = Q K^T, operands in shared memory, and O += P V, the
 // weights P taken from tensor memory, where they replace S.  The cache's codes become halves on the way into shared memory (exact); keys
-// and values have one layout there, rows of 64 dims with the 128-byte swizzle: K-major for S, and for O read along the tokens.
+// and values have one layout there, columns of 64 dims with the 128-byte swizzle: K-major for S, and for O read along the tokens.
 //   warps     0..3, 4..7 a row tile of 128 each: a thread has a row, computes its weights and, when their reference moves, rescales O;
-//             then four that convert keys and values, two buffers each; then one that issues the products.  While one row tile's weights
-//             are computed the tensor core has the other's products.
+//             then four that convert keys and values, four buffers each; then one that issues the products
+//   S         has two buffers a row tile: the scores of a tile are there before the weights of the one before are done.  (One buffer of 128
+//             keys reads the queries half as often: 375 us for the prompt below, but 107 for the chunks.)
 //   F32 rows  queries and weights are two halves each: one row tile, and twice the products
-//   TMEM      [0, 256): S (and P) of the row tiles, [256, 512): O; F32: [128, 192) the weights' second halves
-// Bound by the exponentials, 16 a clock, beside the tensor core: 128 x 128 weights take as long as their two products of 128 dims.
-// Every wait is bounded.
+//   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32), O from 128 on; F32: [256, 320) the second halves of P
+// Bound by the exponentials (16 a clock beside those on the multiply-add pipe) and by shared memory: the products read 48 KB a tile and row
+// tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 403 us = 683 TFLOP/s, of which a sixth goes into a block's
+// start and end; ragged chunks of up to 333 tokens, 32 heads over 4 of 64, behind up to 8192: 98 us.  Every wait is bounded.
 #include <algorithm>
 #include "kv8_attn.cuh"
 #include "ts_gemm.cuh"
 
 namespace msb {
 
-constexpr int kKmKeys = 128, kKmRows = 128;      // (kKmStep in kv8_attn.cu)
+constexpr int kKmKeys = kKv8ManyStep, kKmRows = 128, kKmStages = 4;
 
 template <class T, int D>
 struct KmShape {
   static constexpr bool kTwo = sizeof(T) == 4;
   static constexpr int kTiles = kTwo ? 1 : 2, kTerms = kTwo ? 2 : 1;
   static constexpr int kSoft = 4 * kTiles, kMma = kSoft + 4, kWarps = kMma + 1;
-  static constexpr int kBytes = 128 * D * 2;                          // a tile of 128 rows as halves
-  static constexpr int kSmem = 3072 + kTiles * kTerms * kBytes + 4 * kBytes;
-  static constexpr uint32_t kO = 256, kLow = 128;
+  static constexpr int kQ = kKmRows * D * 2, kKv = kKmKeys * D * 2;      // bytes of a row tile's queries (a term), of a tile's keys or values
+  static constexpr int kSmem = 4096 + kTiles * kTerms * kQ + 2 * kKmStages * kKv;
+  static constexpr uint32_t kO = 128, kLow = 256;
 };
 struct KmHead {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2][2], ahalf[2], ofull[2], qfull;      // pfull: of a tile's first and second 64 keys
+  uint64_t kfull[kKmStages], kempty[kKmStages], vfull[kKmStages], vempty[kKmStages];
+  uint64_t sfull[2][2], pfull[2][2], odone[2], ofull[2], qfull;        // [row tile][buffer]; odone: after each tile but the last, ofull: after that
   uint32_t tmem_base;
   int abort_flag;
   float f0[2 * kKmRows];
-  float4 sc[2][kKmKeys / 16];       // key scale, exponent of the value scale, its inverse; of 16 tokens of a tile
+  float4 sc[kKmStages][kKmKeys / 16];       // key scale, exponent of the value scale, its inverse; of 16 tokens of a tile
 };
-static_assert(sizeof(KmHead) <= 2048, "the tiles follow");
+static_assert(sizeof(KmHead) <= 3072, "the tiles follow");
 
 // place of the 16 bytes `j` of row r, 64 halves a row: 8-row groups of 1024 bytes, 128-byte swizzle
 __device__ __forceinline__ uint32_t km_at(int r, int j) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((j ^ (r & 7)) << 4)); }
@@ -84,9 +87,9 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
   extern __shared__ __align__(1024) uint8_t km_smem_raw[];
   uint8_t* smem = km_smem_raw + ((1024u - (smem_u32(km_smem_raw) & 1023u)) & 1023u);
   KmHead* hd = reinterpret_cast<KmHead*>(smem);
-  uint8_t* qs_mem = smem + 2048;                                       // [tiles][terms][kBytes]
-  uint8_t* kmem = qs_mem + S::kTiles * S::kTerms * S::kBytes;          // [2][kBytes]
-  uint8_t* vmem = kmem + 2 * S::kBytes;
+  uint8_t* qs_mem = smem + 3072;                                       // [tiles][terms][kQ]
+  uint8_t* kmem = qs_mem + S::kTiles * S::kTerms * S::kQ;              // [stages][kKv]
+  uint8_t* vmem = kmem + kKmStages * S::kKv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
@@ -101,9 +104,12 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
   if (k0 >= k1) return;
   const int n = (k1 - k0 + kKmKeys - 1) / kKmKeys;
   if (tid == 0) {
-    for (int s = 0; s < 2; s++) {
+    for (int s = 0; s < kKmStages; s++) {
       mbar_init(&hd->kfull[s], 4); mbar_init(&hd->kempty[s], 1); mbar_init(&hd->vfull[s], 4); mbar_init(&hd->vempty[s], 1);
-      mbar_init(&hd->sfull[s], 1); mbar_init(&hd->pfull[s][0], 4); mbar_init(&hd->pfull[s][1], 4); mbar_init(&hd->ahalf[s], 1); mbar_init(&hd->ofull[s], 1);
+    }
+    for (int t = 0; t < 2; t++) {
+      for (int s = 0; s < 2; s++) { mbar_init(&hd->sfull[t][s], 1); mbar_init(&hd->pfull[t][s], 4); }
+      mbar_init(&hd->odone[t], 1); mbar_init(&hd->ofull[t], 1);
     }
     mbar_init(&hd->qfull, 4 * nt);
     hd->abort_flag = 0;
@@ -127,132 +133,152 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     constexpr uint32_t base = (1u << 4) | ((uint32_t)(kKmRows >> 4) << 24);
     constexpr uint32_t is = base | ((uint32_t)(kKmKeys >> 3) << 17), io = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     const bool leader = elect_one();
-    const uint64_t q_d = ts_desc(smem_u32(qs_mem)), k_d = ts_desc(smem_u32(kmem)), v_d = km_desc_mn(smem_u32(vmem), 16384);
+    const uint64_t q_d = ts_desc(smem_u32(qs_mem)), k_d = ts_desc(smem_u32(kmem)), v_d = km_desc_mn(smem_u32(vmem), kKmKeys * 128);
     bool ok = wait(&hd->qfull, 0, kDevWaitFull);
-    // round j: the output's products of tile j, then the scores of tile j + 1 (one copy of the code: it has to stay in the instruction cache)
+    // round j: the scores of tile j + 1, then the output's products of tile j (one copy of the code: it has to stay in the instruction cache)
 #pragma unroll 1
     for (int j = -1; ok && j < n; j++) {
-      const int s = j & 1;
-      const bool more = j + 1 < n;
-      ok = j < 0 || wait(&hd->vfull[s], j >> 1, kDevWaitFull);
-#pragma unroll 1
-      for (int t = 0; ok && t < nt; t++) {
-#pragma unroll 1
-        for (int h = 0; j >= 0 && h < 2; h++) {
-          ok = wait(&hd->pfull[t][h], j, kDevWaitFull);
-          if (!ok) break;
-          ts_fence_after();
-          if (leader) {
-#pragma unroll
-            for (int e = 0; e < S::kTerms; e++)
-#pragma unroll
-              for (int k = 0; k < kKmKeys / 32; k++)
-                ts_mma_f16(tmem + S::kO + t * D, tmem + (e ? S::kLow : t * 128) + h * 32 + k * 8,
-                           v_d + (uint32_t)(s * (S::kBytes >> 4) + h * 512 + k * 128), io, (j | h | e | k) ? 1u : 0u);
-            if (h == 0) ts_commit(&hd->ahalf[t]);
-          }
-          __syncwarp();
-        }
-        ok = ok && (t || !more || wait(&hd->kfull[s ^ 1], (j + 1) >> 1, kDevWaitFull));
+      if (j + 1 < n) {
+        const int s = (j + 1) % kKmStages, b = (j + 1) & 1;
+        ok = wait(&hd->kfull[s], (j + 1) / kKmStages, kDevWaitFull);
         if (!ok) break;
         ts_fence_after();
         if (leader) {
-          if (more) {
+#pragma unroll 1
+          for (int t = 0; t < nt; t++) {
 #pragma unroll
             for (int e = 0; e < S::kTerms; e++)
 #pragma unroll
-              for (int k = 0; k < D / 16; k++) {
-                constexpr uint32_t step[2] = {16384 >> 4, 32 >> 4};
-                const uint32_t o = (k >> 2) * step[0] + (k & 3) * step[1];
-                km_mma_ss(tmem + t * 128, q_d + ((t * S::kTerms + e) * (S::kBytes >> 4) + o), k_d + ((s ^ 1) * (S::kBytes >> 4) + o), is, (e | k) ? 1u : 0u);
-              }
-            ts_commit(&hd->sfull[t]);
-          } else {
-            ts_commit(&hd->ofull[t]);
+              for (int k = 0; k < D / 16; k++)
+                km_mma_ss(tmem + t * 256 + b * kKmKeys, q_d + (uint32_t)((t * S::kTerms + e) * (S::kQ >> 4) + (k >> 2) * (16384 >> 4) + (k & 3) * 2),
+                          k_d + (uint32_t)(s * (S::kKv >> 4) + (k >> 2) * (kKmKeys * 128 >> 4) + (k & 3) * 2), is, (e | k) ? 1u : 0u);
+            ts_commit(&hd->sfull[t][b]);
           }
+          ts_commit(&hd->kempty[s]);
         }
         __syncwarp();
       }
-      if (ok && leader) {
-        if (j >= 0) ts_commit(&hd->vempty[s]);
-        if (more) ts_commit(&hd->kempty[s ^ 1]);
+      if (j < 0) continue;
+      const int s = j % kKmStages, b = j & 1;
+      ok = wait(&hd->vfull[s], j / kKmStages, kDevWaitFull);
+#pragma unroll 1
+      for (int t = 0; ok && t < nt; t++) {
+        ok = wait(&hd->pfull[t][b], j >> 1, kDevWaitFull);
+        if (!ok) break;
+        ts_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int e = 0; e < S::kTerms; e++)
+#pragma unroll
+            for (int k = 0; k < kKmKeys / 16; k++)
+              ts_mma_f16(tmem + t * 256 + S::kO, tmem + (e ? S::kLow + b * 32 : t * 256 + b * kKmKeys) + k * 8,
+                         v_d + (uint32_t)(s * (S::kKv >> 4) + k * (2048 >> 4)), io, (j | e | k) ? 1u : 0u);
+          ts_commit(j + 1 < n ? &hd->odone[t] : &hd->ofull[t]);
+        }
+        __syncwarp();
       }
+      if (ok && leader) ts_commit(&hd->vempty[s]);
       __syncwarp();
     }
   } else if (warp >= S::kSoft && warp < S::kMma) {
     // ------------------------------------------------------------------ codes -> halves
-    constexpr int kPer = D / 16, kRows = 128 / kPer;   // 16-byte pieces a thread has of a tile, kRows rows apart
+    constexpr int kPer = D / 16, kRows = 128 / kPer;   // 16-byte pieces a thread has of two tiles, kRows rows apart
     // a quarter of a warp has two rows' pieces of one 64-dim half: its stores meet no bank twice
     const int c = tid - S::kSoft * 32, pc = D == 128 ? (c & 3) | (c >> 1 & 4) : c & 3, row0 = D == 128 ? (c >> 2 & 1) | (c >> 4) << 1 : c >> 2;
     const int* table = p.b.table + (size_t)blockIdx.y * p.b.table_stride;
     const int mask = (1 << p.c.shift) - 1;
-    const uint32_t at0 = (pc >> 2) * 16384 + km_at(row0, 2 * (pc & 3)), at1 = (pc >> 2) * 16384 + km_at(row0, 2 * (pc & 3) + 1);
-    // blocks of 16 tokens a lane, of the tile being put and of the next one: every load has a tile's time to arrive (nothing looks at an
-    // id before it is used)
+    const uint32_t at0 = (pc >> 2) * (kKmKeys * 128) + km_at(row0, 2 * (pc & 3)), at1 = (pc >> 2) * (kKmKeys * 128) + km_at(row0, 2 * (pc & 3) + 1);
+    // blocks of 16 tokens a lane, of the two tiles being put and of the next two: every load has two tiles' time to arrive (nothing looks
+    // at an id before it is used)
     constexpr int kNone = -2147483647 - 1;
     auto look_up = [&](int j) {
-      const int key = k0 + kKmKeys * j + 16 * lane;
-      return lane < kKmKeys / 16 && key < k1 ? __ldg(table + (key >> p.c.shift)) : kNone;
+      const int key = k0 + 2 * kKmKeys * j + 16 * lane;
+      return lane < 2 * kKmKeys / 16 && key < k1 ? __ldg(table + (key >> p.c.shift)) : kNone;
     };
-    auto load = [&](uint4 (&r)[kPer], const uint8_t* codes, int ids, int j) {
+    // every load is made, from the first block where there is none and of rows behind the last token (which hold anything): without branches
+    // between them they leave one after the other.  What is not there becomes zeros when it is put.
+    uint32_t low[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; i++) low[i] = (uint32_t)(((k0 + row0 + i * kRows) & mask) * D + pc * 16);      // (128 keys a round)
+    uint4 rk[kPer], rv[kPer];
+    auto load = [&](uint4 (&r)[kPer], const uint8_t* codes, int ids) {
       // head of the block, in units of 1024 bytes (a block of a head is 1024 at least)
-      const uint32_t head = ids < 0 ? 0xFFFFFFFFu : (uint32_t)(((((uint64_t)ids * p.c.heads + kvh) << p.c.shift) * D) >> 10);
-      const int rows = sq.len - (k0 + kKmKeys * j);    // rows behind the last token hold anything
+      const uint32_t head = (uint32_t)(((((uint64_t)max(ids, 0) * p.c.heads + kvh) << p.c.shift) * D) >> 10);
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
-        const int row = row0 + i * kRows;
-        const uint32_t h = __shfl_sync(0xffffffffu, head, row >> 4);
-        r[i] = make_uint4(0, 0, 0, 0);
-        if (h != 0xFFFFFFFFu && row < rows) r[i] = __ldg(reinterpret_cast<const uint4*>(codes + ((uint64_t)h << 10) + (row & mask) * D) + pc);
+        const uint32_t h = __shfl_sync(0xffffffffu, head, (row0 + i * kRows) >> 4);
+        r[i] = __ldg(reinterpret_cast<const uint4*>(codes + ((uint64_t)h << 10) + low[i]));
       }
     };
-    auto put = [&](uint8_t* dst, const uint4 (&r)[kPer]) {
+    auto put = [&](uint8_t* dst, uint4 (&r)[kPer], int half, int ids, int j) {
+      const int rows = sq.len - (k0 + 2 * kKmKeys * j);
+      if (rows < 2 * kKmKeys || __any_sync(0xffffffffu, lane < 2 * kKmKeys / 16 && ids < 0)) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+          const int row = row0 + i * kRows, id = __shfl_sync(0xffffffffu, ids, row >> 4);
+          if (i / (kPer / 2) == half && (id < 0 || row >= rows)) r[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kPer; i++) {
-        *reinterpret_cast<uint4*>(dst + at0 + i * kRows * 128) = make_uint4(kv8_half2(r[i].x), kv8_half2(r[i].x >> 16), kv8_half2(r[i].y), kv8_half2(r[i].y >> 16));
-        *reinterpret_cast<uint4*>(dst + at1 + i * kRows * 128) = make_uint4(kv8_half2(r[i].z), kv8_half2(r[i].z >> 16), kv8_half2(r[i].w), kv8_half2(r[i].w >> 16));
+        if (i / (kPer / 2) != half) continue;
+        const int o = (i % (kPer / 2)) * kRows * 128;
+        *reinterpret_cast<uint4*>(dst + at0 + o) = make_uint4(kv8_half2(r[i].x), kv8_half2(r[i].x >> 16), kv8_half2(r[i].y), kv8_half2(r[i].y >> 16));
+        *reinterpret_cast<uint4*>(dst + at1 + o) = make_uint4(kv8_half2(r[i].z), kv8_half2(r[i].z >> 16), kv8_half2(r[i].w), kv8_half2(r[i].w >> 16));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     };
     const bool scales = warp == S::kSoft;
-    uint4 rk[kPer], rv[kPer];
     int ids = -1, next = look_up(0);
     float ks = 0.f, vs = 1.f;
-    // round j: tile j from registers into shared memory, tile j + 1 into the registers
+    // round j: tiles 2 j and 2 j + 1 from registers into shared memory, the next two into the registers
+    const int rounds = (n + 1) / 2;
+    bool ok = true;
 #pragma unroll 1
-    for (int j = -1; j < n; j++) {
-      const int s = j & 1;
-      const bool more = j + 1 < n;
+    for (int j = -1; ok && j < rounds; j++) {
+      const bool more = j + 1 < rounds;
       if (j >= 0) {
-        if (!wait(&hd->kempty[s], (j >> 1) ^ 1, kDevWaitEmpty)) break;
-        put(kmem + s * S::kBytes, rk);
-        if (lane == 0) mbar_arrive(&hd->kfull[s]);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int i = 2 * j + h, s = i % kKmStages;
+          if (!ok || i >= n) break;
+          ok = wait(&hd->kempty[s], (i / kKmStages) ^ 1, kDevWaitEmpty);
+          if (!ok) break;
+          put(kmem + s * S::kKv, rk, h, ids, j);
+          if (lane == 0) mbar_arrive(&hd->kfull[s]);
+        }
       }
       if (more) {
         if (next < 0 || next >= p.c.n_blocks) {
           if (next != kNone) atomicCAS(p.status, 0, kDevBadBatch);
           next = -1;
         }
-        load(rk, p.c.k, next, j + 1);
+        load(rk, p.c.k, next);
       }
       if (j >= 0) {
-        if (!wait(&hd->vempty[s], (j >> 1) ^ 1, kDevWaitEmpty)) break;     // with it the scales of two tiles ago have been used
-        if (scales && lane < kKmKeys / 16) {
-          const int e = kv8_exp(vs);
-          hd->sc[s][lane] = ids < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(ks, (float)e, kv8_pow2(-e), 0.f);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int i = 2 * j + h, s = i % kKmStages;
+          if (!ok || i >= n) break;
+          ok = wait(&hd->vempty[s], (i / kKmStages) ^ 1, kDevWaitEmpty);   // with it the scales of four tiles ago have been used
+          if (!ok) break;
+          if (scales && lane / (kKmKeys / 16) == h) {
+            const int e = kv8_exp(vs);
+            hd->sc[s][lane % (kKmKeys / 16)] = ids < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(ks, (float)e, kv8_pow2(-e), 0.f);
+          }
+          put(vmem + s * S::kKv, rv, h, ids, j);
+          if (lane == 0) mbar_arrive(&hd->vfull[s]);
         }
-        put(vmem + s * S::kBytes, rv);
-        if (lane == 0) mbar_arrive(&hd->vfull[s]);
       }
       if (more) {
-        load(rv, p.c.v, next, j + 1);
+        load(rv, p.c.v, next);
         if (scales && next >= 0) {
           ks = __ldg(p.c.ks + (size_t)next * p.c.heads + kvh);
           vs = __ldg(p.c.vs + (size_t)next * p.c.heads + kvh);
         }
         ids = next;
-        next = j + 2 < n ? look_up(j + 2) : kNone;
+        next = j + 2 < rounds ? look_up(j + 2) : kNone;
       }
     }
   } else if (warp < S::kSoft && (warp >> 2) < nt) {
@@ -265,7 +291,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     {
       // the warp's 32 rows, D / 8 lanes a row: their largest, then halves.  A logit in binary exponents is product * f0 * key scale
       constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
-      uint8_t* dst = qs_mem + t * S::kTerms * S::kBytes;
+      uint8_t* dst = qs_mem + t * S::kTerms * S::kQ;
       const int c = lane % kLanes, dq = kAtOnce / p.G, dr = kAtOnce % p.G;
       constexpr int kBatch = TWO ? 4 : 8;              // rows requested at once
       int rr = w0 + lane / kLanes, tk = rr / p.G, hh = rr - tk * p.G;        // row, token, head of the group
@@ -313,7 +339,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           }
           uint8_t* q = dst + (c >> 3) * 16384 + km_at((warp & 3) * 32 + r, c & 7);
           *reinterpret_cast<uint4*>(q) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (TWO) *reinterpret_cast<uint4*>(q + S::kBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (TWO) *reinterpret_cast<uint4*>(q + S::kQ) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -321,19 +347,21 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
       if (lane == 0) mbar_arrive(&hd->qfull);
     }
     const float f0 = hd->f0[t * 128 + tr];
-    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + t * 128, to = tmem + lanes + S::kO + t * D;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, to = tmem + lanes + t * 256 + S::kO;
     const int first = p.window ? max(0, pos - p.window + 1) : 0, last = min(k1 - 1, pos);      // keys that the row sees
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+#pragma unroll 1
     for (int j = 0; j < n; j++) {
-      const int s = j & 1, base = k0 + kKmKeys * j;
-      ok = wait(&hd->sfull[t], j, kDevWaitFull) && wait(&hd->vfull[s], j >> 1, kDevWaitFull);     // the tile's scales come with its values
+      const int s = j % kKmStages, base = k0 + kKmKeys * j;
+      const uint32_t ts = tmem + lanes + t * 256 + (j & 1) * kKmKeys;
+      ok = wait(&hd->sfull[t][j & 1], j >> 1, kDevWaitFull) && wait(&hd->vfull[s], j / kKmStages, kDevWaitFull);     // the scales come with the values
       if (!ok) break;
       __syncwarp();
       ts_fence_after();
       const bool cut = base + kKmKeys > all_hi || base < all_lo;
       float mm = m == -INFINITY ? 0.f : m;
-      if (__any_sync(0xffffffffu, m == -INFINITY)) {   // no reference yet: the tile's largest exponent (that of its first 16 keys had to move later)
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {   // no reference yet: the tile's largest exponent
         float top = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < kKmKeys / 16; c++) {
@@ -351,22 +379,20 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
         if (m == -INFINITY) m = top;
         mm = m == -INFINITY ? 0.f : m;
       }
-      // ---- weights, 64 keys at a time, into columns of products that have been read.  The reference stays unless the weights of 16 keys
-      // sum to more than 2^15 (a half holds each of them then): it moves up by a whole number, what has been summed against the old one is
-      // scaled, and the 64 weights are made again
-      float sum = 0.f;
+      // ---- weights.  The reference stays unless the weights of 16 keys sum to more than 60000 (a half holds each of them below that): it moves up
+      // by a whole number, what has been summed against the old one is scaled, and the weights are made again
       bool lost = false;
       int tries = 0;
+      uint32_t w[4][16];
+      float part[4];
 #pragma unroll 1
-      for (int c = 0; c < kKmKeys / 16;) {             // (unrolled, its code no longer stays in the instruction cache)
-        uint32_t w[4][16];
-        float part[4];
+      for (;;) {
 #pragma unroll
-        for (int h = 0; h < 4; h++) ts_ld16(ts + 16 * (c + h), w[h]);
+        for (int h = 0; h < 4; h++) ts_ld16(ts + 16 * h, w[h]);
         ts_wait_ld();
 #pragma unroll
         for (int h = 0; h < 4; h++) {
-          const float4 sc = hd->sc[s][c + h];
+          const float4 sc = hd->sc[s][h];
           const uint64_t f = kv8_two(f0 * sc.x, f0 * sc.x), b = kv8_two(sc.y - mm, sc.y - mm);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
@@ -376,7 +402,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           }
         }
         if (cut) {
-          const int hi = last - base - 16 * c, lo = first - base - 16 * c;
+          const int hi = last - base, lo = first - base;
 #pragma unroll
           for (int i = 0; i < 64; i++)
             if (i > hi || i < lo) w[i >> 4][i & 15] = 0xFF800000u;
@@ -398,105 +424,128 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           part[h] = y + z;
         }
         const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        if (__any_sync(0xffffffffu, most > 32768.f && !lost)) {
-          // to the next power of two above the sum, or, where that is beyond 32 bits, to the largest exponent.  A row whose products
-          // are infinite has none, and beyond 2^35 exponents are too coarse for one: after four times its weights stay what they are
-          float up = most > 32768.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) : 0.f;
-          if (__any_sync(0xffffffffu, up > 128.f)) {
-            float top = -INFINITY;
+        if (!__any_sync(0xffffffffu, most > 60000.f && !lost)) break;
+        // to the next power of two above the sum, or, where that is beyond 32 bits, to the largest exponent.  A row whose products are
+        // infinite has none, and beyond 2^35 exponents are too coarse for one: after four times its weights stay what they are
+        float up = most > 60000.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) : 0.f;
+        if (__any_sync(0xffffffffu, up > 128.f)) {
+          float top = -INFINITY;
 #pragma unroll 1
-            for (int k = 0; k < 4; k++) {
-              ts_ld16(ts + 16 * (c + k), w[0]);
-              ts_wait_ld();
-              const float4 sc = hd->sc[s][c + k];
+          for (int k = 0; k < 4; k++) {
+            ts_ld16(ts + 16 * k, w[0]);
+            ts_wait_ld();
+            const float4 sc = hd->sc[s][k];
 #pragma unroll
-              for (int i = 0; i < 16; i++) {
-                const int key = base + 16 * (c + k) + i;
-                if (!cut || (key >= first && key <= last)) top = fmaxf(top, fmaf(__uint_as_float(w[0][i]), f0 * sc.x, sc.y - mm));
-              }
-              __syncwarp();
+            for (int i = 0; i < 16; i++) {
+              const int key = base + 16 * k + i;
+              if (!cut || (key >= first && key <= last)) top = fmaxf(top, fmaf(__uint_as_float(w[0][i]), f0 * sc.x, sc.y - mm));
             }
-            if (up > 128.f) {
-              lost = !(top < INFINITY);
-              up = lost ? 0.f : ceilf(top);
-            }
-          }
-          if (++tries == 4) lost = true;
-          const float f = km_exp2(-up);
-          m += up; mm = m; l *= f; sum *= f;
-          if (j | c) {
-            // the sums so far: with the first 64 weights of this tile, once their products are there
-            if (c) ok = wait(&hd->ahalf[t], j, kDevWaitFull);
-            if (!ok) break;
             __syncwarp();
-            ts_fence_after();
+          }
+          if (up > 128.f) {
+            lost = !(top < INFINITY);
+            up = lost ? 0.f : ceilf(top);
+          }
+        }
+        if (++tries == 4) lost = true;
+        const float f = km_exp2(-up);
+        m += up; mm = m; l *= f;
+        if (j) {                                       // the products of the tile before are there (those of two before are: this tile's scores are)
+          ok = wait(&hd->odone[t], j - 1, kDevWaitFull);
+          if (!ok) break;
+          __syncwarp();
+          ts_fence_after();
 #pragma unroll 1
-            for (int k = 0; k < D / 16; k++) {
-              ts_ld16(to + 16 * k, w[0]);
-              ts_wait_ld();
+          for (int k = 0; k < D / 16; k++) {
+            ts_ld16(to + 16 * k, w[0]);
+            ts_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; i++) w[0][i] = __float_as_uint(__uint_as_float(w[0][i]) * f);
-              ts_st16(to + 16 * k, w[0]);
-            }
+            for (int i = 0; i < 16; i++) w[0][i] = __float_as_uint(__uint_as_float(w[0][i]) * f);
+            ts_st16(to + 16 * k, w[0]);
           }
           ts_wait_st();
-          continue;
         }
-#pragma unroll
-        for (int h = 0; h < 4; h++) sum = fmaf(part[h], hd->sc[s][c + h].z, sum);
-#pragma unroll
-        for (int h = 0; h < 4; h += 2) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float u = __uint_as_float(w[h + (i >> 3)][2 * i & 15]), v = __uint_as_float(w[h + (i >> 3)][(2 * i & 15) + 1]);
-            hi[i] = km_pack(u, v);
-            if (TWO) {
-              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-              lo[i] = km_pack(u - y.x, v - y.y);
-            }
-          }
-          ts_st16(ts + 8 * (c + h), hi);
-          if constexpr (TWO) ts_st16(tmem + lanes + S::kLow + 8 * (c + h), lo);
-        }
-        ts_wait_st();
-        ts_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&hd->pfull[t][c >> 2]);
-        c += 4;
-        tries = 0;
       }
       if (!ok) break;
-      l += sum;
+#pragma unroll
+      for (int h = 0; h < 4; h++) l = fmaf(part[h], hd->sc[s][h].z, l);
+#pragma unroll
+      for (int h = 0; h < 4; h += 2) {                 // in place of the products, all of which have been read
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float u = __uint_as_float(w[h + (i >> 3)][2 * i & 15]), v = __uint_as_float(w[h + (i >> 3)][(2 * i & 15) + 1]);
+          hi[i] = km_pack(u, v);
+          if (TWO) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+            lo[i] = km_pack(u - y.x, v - y.y);
+          }
+        }
+        ts_st16(ts + 8 * h, hi);
+        if constexpr (TWO) ts_st16(tmem + lanes + S::kLow + (j & 1) * 32 + 8 * h, lo);
+      }
+      ts_wait_st();
+      ts_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&hd->pfull[t][j & 1]);
     }
-    if (ok) ok = wait(&hd->ofull[t], 0, kDevWaitFull);
+    ok = ok && wait(&hd->ofull[t], 0, kDevWaitFull);
     if (ok) {
       __syncwarp();
       ts_fence_after();
-      const bool last = p.splits == 1;
+      const bool whole = p.splits == 1;
+      const size_t at = ((size_t)split * p.b.n_tokens + sq.row + tok) * p.heads + head;
       float mul = 1.f;
-      if (last) {
+      if (whole) {
         float sum = l;
         if (p.sinks) sum += km_exp2(p.sinks[head] * kLog2e - (m == -INFINITY ? 0.f : m));
         mul = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
+      } else if (live) {
+        *reinterpret_cast<float2*>(kv8_part_ml(p, D) + 2 * at) = make_float2(m, l);
       }
-      const size_t at = ((size_t)split * p.b.n_tokens + sq.row + tok) * p.heads + head;
-      if (!last && live) *reinterpret_cast<float2*>(kv8_part_ml(p, D) + 2 * at) = make_float2(m, l);
+      // a row to the place of its queries (which nothing reads any more), then whole rows at a time to memory
+      constexpr int kRowBytes = D * sizeof(T), kPieces = kRowBytes / 16;
+      uint8_t* rows = qs_mem + (t * kKmRows + (warp & 3) * 32) * kRowBytes;
 #pragma unroll 1
       for (int c = 0; c < D / 16; c++) {
         uint32_t a[16];
         __syncwarp();
         ts_ld16(to + 16 * c, a);
         ts_wait_ld();
-        if (live) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            float v[8];
+        for (int h = 0; h < 2; h++) {
+          float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = __uint_as_float(a[8 * h + i]) * mul;
-            if (last) Elems<T>::store(static_cast<T*>(p.out) + (sq.row + tok) * p.out_stride + (int64_t)head * D + 16 * c + 8 * h, p.out_vec, v);
-            else Elems<float>::store(p.part + at * D + 16 * c + 8 * h, true, v);
+          for (int i = 0; i < 8; i++) v[i] = __uint_as_float(a[8 * h + i]) * mul;
+          if (whole) {
+            const int o = (2 * c + h) * (8 * sizeof(T) / 16);
+#pragma unroll
+            for (int k = 0; k < (int)(8 * sizeof(T) / 16); k++)
+              *reinterpret_cast<uint4*>(rows + lane * kRowBytes + (((o + k) ^ (lane & 7)) << 4)) = Elems<T>::pack16(v, k);
+          } else if (live) {
+            Elems<float>::store(p.part + at * D + 16 * c + 8 * h, true, v);
           }
+        }
+      }
+      if (whole) {
+        __syncwarp();
+        const int64_t mine = (sq.row + tok) * p.out_stride + (int64_t)head * D;
+#pragma unroll 4
+        for (int i = 0; i < kPieces; i++) {            // 32 pieces of the warp's 32 rows at a time
+          const int c = i * 32 + lane, r = c / kPieces, pc = c % kPieces;
+          const int64_t o = __shfl_sync(0xffffffffu, mine, r);
+          if (w0 + r < R) {
+            T* dst = static_cast<T*>(p.out) + o + pc * (16 / (int)sizeof(T));
+            const uint4 u = *reinterpret_cast<const uint4*>(rows + r * kRowBytes + ((pc ^ (r & 7)) << 4));
+            if (p.out_vec) {
+              *reinterpret_cast<uint4*>(dst) = u;
+            } else {
+              const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+              for (int k = 0; k < (int)(16 / sizeof(T)); k++) dst[k] = e[k];
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -523,7 +572,7 @@ static int launch_many(const Kv8AttnParams& p, int groups, cudaStream_t st, int 
   MSB_LAUNCH_CHECK("kv8_attn");
   return kOk;
 }
-int kv8_many_rows(int elem_type) { return elem_type == F32 ? kKmRows : 2 * kKmRows; }
+static_assert(kKv8ManyRowsF32 == kKmRows && kKv8ManyRows == 2 * kKmRows, "row tiles of a block");
 int kv8_attn_many(const Kv8AttnParams& p, int groups, int elem_type, int D, cudaStream_t st, int dev) {
   if (elem_type == F32) return D == 64 ? launch_many<float, 64>(p, groups, st, dev) : launch_many<float, 128>(p, groups, st, dev);
   if (elem_type == F16) return D == 64 ? launch_many<__half, 64>(p, groups, st, dev) : launch_many<__half, 128>(p, groups, st, dev);

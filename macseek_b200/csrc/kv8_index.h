@@ -70,18 +70,47 @@ inline int kv8_span(int max_len, int rows, int G, int window, int step) {
   return window && w < max_len ? (int)w : max_len;
 }
 
-// Split of the keys: `units` blocks of threads without one, about `want` blocks wanted; chunks of at least `least` keys, a multiple of `step`.
-struct Kv8Split { int chunk, splits; };
-inline Kv8Split kv8_split(int span, int64_t units, int64_t want, int least, int step = 64) {
-  const int64_t n = want / (units > 0 ? units : 1) > 1 ? want / units : 1;
-  int64_t chunk = ((span + n - 1) / n + step - 1) / step * step;
-  if (chunk < least) chunk = least;
-  return Kv8Split{(int)chunk, (int)((span + chunk - 1) / chunk)};
+// How a call of the attention runs: on the kernel for few rows (blocks of 16 rows of a key head, all of them reading the keys) or on the one
+// for many (256, F32 128), and in how many parts the keys are split.  The estimate of a call, in us, from times on a B200: blocks an SM at a
+// time, their start, their keys, and for parts the join, which reads what they wrote.  Of sequences whose lengths differ 0.6 are counted.
+struct Kv8Plan { int many, rows, step, tiles, chunk, splits; };
+constexpr int kKv8FewRows = 16, kKv8FewStep = 32, kKv8ManyRows = 256, kKv8ManyRowsF32 = 128, kKv8ManyStep = 64, kKv8Least = 128;
+
+// splits at most of either kernel, whatever the window
+struct Kv8Most { int few, many; };
+inline Kv8Most kv8_most(int n_seq, int max_new, int max_len, int kv_heads, int heads, bool f32, int sms) {
+  const int64_t rows = (int64_t)max_new * (heads / kv_heads), groups = (int64_t)n_seq * kv_heads, full = (max_len + kKv8Least - 1ll) / kKv8Least;
+  const int64_t few = 3ll * sms * (n_seq > 1 ? 6 : 1) / ((rows + kKv8FewRows - 1) / kKv8FewRows * groups);
+  const int many_rows = f32 ? kKv8ManyRowsF32 : kKv8ManyRows;
+  const int64_t many = 4ll * sms / ((rows + many_rows - 1) / many_rows * groups);
+  return Kv8Most{(int)(few < 1 ? 1 : few < full ? few : full), (int)(many < 1 ? 1 : many < full ? many : full)};
 }
-// splits that kv8_split never exceeds for any span up to max_len
-inline int kv8_most_splits(int max_len, int64_t units, int64_t want, int least) {
-  const int64_t n = want / (units > 0 ? units : 1) > 1 ? want / units : 1, m = ((int64_t)max_len + least - 1) / least;
-  return (int)(n < m ? n : m);
+inline Kv8Plan kv8_plan(int n_seq, int max_new, int max_len, int kv_heads, int heads, int dim, bool f32, int window, int sms) {
+  const int G = heads / kv_heads;
+  const int64_t rows = (int64_t)max_new * G, groups = (int64_t)n_seq * kv_heads;
+  const double part = n_seq > 1 ? 0.6 : 1.0, joined = part * n_seq * max_new * heads * (dim + 2) * 8 / 4e6;      // us a part: written, read
+  const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const Kv8Most most = kv8_most(n_seq, max_new, max_len, kv_heads, heads, f32, sms);
+  double best[2] = {0, 0};
+  Kv8Plan plans[2] = {{0, kKv8FewRows, kKv8FewStep, 0, 0, 0}, {1, f32 ? kKv8ManyRowsF32 : kKv8ManyRows, kKv8ManyStep, 0, 0, 0}};
+  for (int k = 0; k < 2; k++) {
+    Kv8Plan& pl = plans[k];
+    const int span = kv8_span(max_len, pl.rows, G, window, pl.step), unit = k ? pl.step : 64, top = k ? most.many : most.few;
+    pl.tiles = (int)up(rows, pl.rows);
+    const int64_t units = pl.tiles * groups;
+    // few: keys of 16 rows that an SM does in a us, by three blocks (one alone: 1 / 1.7 of them); many: us a key of a block's rows
+    const double speed = f32 ? (dim == 64 ? 182 : 81) : (dim == 64 ? 230 : 155), per_key = f32 ? (dim == 64 ? 0.032 : 0.044) : (dim == 64 ? 0.031 : 0.034);
+    for (int n = 1, last = 0; n <= top; n++) {
+      const int chunk = kv8_max((int)(up(up(span, n), unit) * unit), kKv8Least), parts = (int)up(span, chunk);
+      if (parts == last) continue;
+      last = parts;
+      const int64_t blocks = (int64_t)(units * parts * part) + 1, at_once = blocks > 2 * sms ? 3 : blocks > sms ? 2 : 1;
+      const double one = k ? 7 + per_key * chunk : 2 + chunk * (at_once > 1 ? at_once : 1.7) / speed;
+      const double us = 4 + (double)up(blocks, k ? sms : 3 * sms) * one + (parts > 1 ? 3 + joined * parts : 0);
+      if (pl.splits == 0 || us < best[k]) { best[k] = us; pl.chunk = chunk; pl.splits = parts; }
+    }
+  }
+  return best[0] <= best[1] ? plans[0] : plans[1];
 }
 
 }  // namespace msb

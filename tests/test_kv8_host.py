@@ -74,17 +74,18 @@ int main() {
       for (int r = 0; r < n_tokens; r++) NEED(seen[r] == (r < start[n_seq]));
     // rows -> sequence, key ranges and their splits
     for (int k = 0; k < 20; k++) {
-      const int s = upto(n_seq - 1), G = 1 + upto(8), window = upto(1) ? 0 : 1 + upto(300), step = 16 << upto(3), rows = 16 << upto(3);
+      const int s = upto(n_seq - 1), G = 1 + upto(8), window = upto(1) ? 0 : 1 + upto(300), kvh = 1 + upto(8);
+      const bool f32 = upto(1);
+      const Kv8Plan pl = kv8_plan(n_seq, max_new, max_len, kvh, kvh * G, 64 << upto(1), f32, window, 148);
+      const Kv8Most most = kv8_most(n_seq, max_new, max_len, kvh, kvh * G, f32, 148);
+      const int step = pl.step, rows = pl.rows;
+      NEED(pl.chunk % step == 0 && pl.chunk > 0 && pl.splits <= (pl.many ? most.many : most.few) && (int64_t)pl.tiles * rows >= (int64_t)max_new * G);
       Kv8Seq q;
       if (!kv8_seq_of(start[s], start[s + 1], len[s], n_tokens, max_new, max_len, q) || q.n == 0) continue;
       if (!broken) {
         const int tok = q.row + upto(q.n - 1);
         NEED(kv8_search(n_seq, tok, [&](int i) { return start[i]; }, Host()) == s);
       }
-      const int span = kv8_span(max_len, rows, G, window, step);
-      const int64_t units = 1 + upto(900), want = 444 * (1 + upto(2));
-      const Kv8Split sp = kv8_split(span, units, want, 128);
-      NEED(sp.chunk % 64 == 0 && sp.splits <= kv8_most_splits(max_len, units, want, 128));
       for (int m0 = 0; m0 < q.n * G; m0 += rows) {
         const int m1 = kv8_min(m0 + rows, q.n * G);
         const Kv8Range r = kv8_range(q, m0, m1, G, window, step);
@@ -93,7 +94,7 @@ int main() {
           const int pos = q.len - q.n + m / G, from = window ? kv8_max(0, pos - window + 1) : 0;
           NEED(r.lo <= from && pos < r.hi);
         }
-        NEED((r.hi - r.lo + sp.chunk - 1) / sp.chunk <= sp.splits);
+        NEED((r.hi - r.lo + pl.chunk - 1) / pl.chunk <= pl.splits);
       }
     }
   }
@@ -108,6 +109,20 @@ def test_index_arithmetic_covers_every_row_once_and_stays_in_bounds(tmp_path):
     subprocess.check_call(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I" + CSRC, str(src), "-o", str(exe)])
     r = subprocess.run([str(exe)], text=True, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     assert r.stdout.strip() == "ok", r.stdout
+
+
+def test_attention_takes_the_kernel_and_the_split_that_end_sooner(tmp_path):
+    # sequences, new rows, tokens, key heads, heads, dim, f32, window -> many rows' kernel, splits of the keys
+    cases = {(1, 1, 1, 8, 64, 128, 0, 0): (0, 1), (1, 1, 999, 8, 64, 128, 1, 0): (0, 8), (1, 1, 200000, 8, 64, 128, 0, 0): (0, 55),
+             (64, 1, 8192, 8, 64, 128, 0, 0): (0, 4), (64, 1, 8192, 8, 64, 128, 0, 128): (0, 1), (16, 4, 4004, 8, 64, 64, 0, 0): (0, 5),
+             (1, 64, 64, 8, 64, 64, 0, 0): (0, 1), (1, 4096, 4096, 8, 64, 128, 0, 0): (1, 1), (1, 4096, 4096, 8, 64, 128, 1, 0): (1, 1),
+             (5, 333, 8525, 4, 32, 64, 0, 4096): (1, 1), (1, 256, 1256, 8, 64, 128, 0, 0): (1, 2), (1, 16, 16016, 8, 64, 128, 1, 0): (1, 18)}
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text('#include "kv8_index.h"\n#include <cstdio>\nint main() {\n' + "\n".join(
+        '{ auto p = msb::kv8_plan(%s, 148); printf("%%d %%d\\n", p.many, p.splits); }' % ", ".join(map(str, c)) for c in cases) + "\n}\n")
+    subprocess.check_call(["g++", "-std=c++17", "-I" + CSRC, str(src), "-o", str(exe)])
+    got = [tuple(int(v) for v in line.split()) for line in subprocess.check_output([str(exe)], text=True).splitlines()]
+    assert dict(zip(cases, got)) == cases
 
 
 # ------------------------------------------------------------------------------------------------ refusals of the C entry points
