@@ -13,6 +13,7 @@
 
 namespace msb {
 
+constexpr int kKdCluster = 8;      // blocks of a cluster at most
 constexpr int kKdWarps = 4, kKdStages = 2, kKdStep = kKv8FewStep, kKdRows = kKv8FewRows;
 
 __device__ __forceinline__ void kd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -52,7 +53,28 @@ struct KdTile {
   }
 };
 
-template <class T, int D>
+__device__ __forceinline__ void kd_cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t kd_of_block(const void* p, uint32_t rank) {      // the same shared variable of another block of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float kd_load_of(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 kd_load4_of(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// CLUSTER: the parts of a row are the blocks of a cluster, which join them through one another's shared memory
+template <class T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv8AttnParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -60,7 +82,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   constexpr int KS = D / 16, NT = D / 8, CH = D / 64;      // k-steps, output tiles, 16-byte chunks of a key row per lane
   constexpr int kHalf = 16 * D, kStage = 4 * kHalf, kWarpBytes = kKdStages * kStage, kPitch = D + 4;     // keys of 32 tokens, their values
   extern __shared__ __align__(16) uint8_t kd_smem[];
-  __shared__ float s_m[kKdWarps][kKdRows], s_l[kKdWarps][kKdRows];
+  __shared__ float s_m[kKdWarps][kKdRows], s_l[kKdWarps][kKdRows], s_bm[kKdRows], s_bl[kKdRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int tiles = gridDim.y / p.c.heads, kvh = blockIdx.y / tiles, m0 = (blockIdx.y % tiles) * kKdRows;
   const Kv8Seq sq = kv8_seq(p.b, blockIdx.z, p.status);
@@ -69,8 +91,8 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   const int m1 = min(m0 + kKdRows, R);
   const Kv8Range kr = kv8_range(sq, m0, m1, p.G, p.window, kKdStep);
   const int k0 = kr.lo + blockIdx.x * p.chunk, k1 = min(kr.hi, k0 + p.chunk);
-  if (k0 >= k1) return;
-  const int steps = (k1 - k0 + kKdStep - 1) / kKdStep;
+  if (!CLUSTER && k0 >= k1) return;
+  const int steps = k1 > k0 ? (k1 - k0 + kKdStep - 1) / kKdStep : 0;
   const int mine = steps > warp ? (steps - warp + kKdWarps - 1) / kKdWarps : 0;
   const int* table = p.b.table + (size_t)blockIdx.z * p.b.table_stride;
 
@@ -325,7 +347,10 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
       for (int j = 0; j < 8; j++) v[j] += src[j];
     }
     const int tok = sq.row + row / p.G, head = kvh * p.G + row % p.G;
-    if (last) {
+    if (CLUSTER) {                             // in place: nobody else reads these eight
+      Elems<float>::store(so + r * kPitch + d, true, v);
+      if (d == 0) { s_bm[r] = M; s_bl[r] = sum; }
+    } else if (last) {
       if (p.sinks) sum += kd_exp2(p.sinks[head] * kLog2e - (M == -INFINITY ? 0.f : M));
       const float inv = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
 #pragma unroll
@@ -336,6 +361,43 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
       Elems<float>::store(p.part + at * D + d, true, v);
       if (d == 0) *reinterpret_cast<float2*>(kv8_part_ml(p, D) + 2 * at) = make_float2(M, sum);
     }
+  }
+  if (CLUSTER) {
+    kd_cluster_sync();
+    const int n = gridDim.x;                   // blocks of the cluster: each writes a share of the rows
+    for (int c = tid + kKdWarps * 32 * blockIdx.x; c < (m1 - m0) * (D / 8); c += kKdWarps * 32 * n) {
+      const int r = c / (D / 8), d = c % (D / 8) * 8, row = m0 + r, tok = sq.row + row / p.G, head = kvh * p.G + row % p.G;
+      float M = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, m[kKdCluster], l[kKdCluster];
+#pragma unroll
+      for (int b = 0; b < kKdCluster; b++) {   // all of them requested before the first is used
+        m[b] = b < n ? kd_load_of(kd_of_block(&s_bm[r], b)) : -INFINITY;
+        l[b] = b < n ? kd_load_of(kd_of_block(&s_bl[r], b)) : 0.f;
+      }
+#pragma unroll
+      for (int b = 0; b < kKdCluster; b++) M = fmaxf(M, m[b]);
+#pragma unroll
+      for (int h = 0; h < kKdCluster; h += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const uint32_t src = kd_of_block(so + r * kPitch + d, min(h + b, n - 1));
+          x[b] = kd_load4_of(src); y[b] = kd_load4_of(src + 16);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const float f = m[h + b] == -INFINITY ? 0.f : kd_exp2(m[h + b] - M);      // (and of a block that is not there)
+          sum += l[h + b] * f;
+          v[0] += x[b].x * f; v[1] += x[b].y * f; v[2] += x[b].z * f; v[3] += x[b].w * f;
+          v[4] += y[b].x * f; v[5] += y[b].y * f; v[6] += y[b].z * f; v[7] += y[b].w * f;
+        }
+      }
+      if (p.sinks) sum += kd_exp2(p.sinks[head] * kLog2e - (M == -INFINITY ? 0.f : M));
+      const float inv = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] *= inv;
+      Elems<T>::store(static_cast<T*>(p.out) + tok * p.out_stride + (int64_t)head * D + d, p.out_vec, v);
+    }
+    kd_cluster_sync();                         // no block leaves while another reads its memory
   }
 }
 
@@ -435,19 +497,27 @@ size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, in
 }
 
 template <class T, int D>
-static int launch_attn(const Kv8AttnParams& p, const Kv8Plan& pl, int elem_type, cudaStream_t st, int dev) {
+static int launch_attn(const Kv8AttnParams& p, const Kv8Plan& pl, int elem_type, cudaStream_t st, int dev, int sms) {
   if (pl.many) {
     const int rc = kv8_attn_many(p, pl.tiles, elem_type, D, st, dev);
     if (rc) return rc;
   } else {
-    auto kern = kv8_attn_few_kernel<T, D>;
     const size_t smem = std::max<size_t>((size_t)kKdWarps * kKdStages * 2 * kKdStep * D, sizeof(float) * kKdWarps * kKdRows * (D + 4));
     static bool done[64] = {};
     if (!done[dev & 63]) {
-      MSB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      MSB_CUDA(cudaFuncSetAttribute(kv8_attn_few_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      MSB_CUDA(cudaFuncSetAttribute(kv8_attn_few_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
       done[dev & 63] = true;
     }
-    MSB_CUDA(launch_pdl(kern, dim3(pl.splits, p.c.heads * pl.tiles, p.b.n_seq), dim3(kKdWarps * 32), smem, st, p));
+    const dim3 grid(pl.splits, p.c.heads * pl.tiles, p.b.n_seq);
+    // few parts of few rows: one launch, the parts a cluster (a token of 64 heads over 8 behind 998: 10.5 -> KD_US us).  Not once the blocks do
+    // not all run at once: those of short sequences would wait for the long ones of their cluster
+    if (pl.splits > 1 && pl.splits <= kKdCluster && (int64_t)grid.x * grid.y * grid.z <= 2 * sms) {
+      MSB_CUDA(launch_clusters(kv8_attn_few_kernel<T, D, true>, grid, dim3(kKdWarps * 32), pl.splits, smem, st, p));
+      MSB_LAUNCH_CHECK("kv8_attn");
+      return kOk;
+    }
+    MSB_CUDA(launch_pdl(kv8_attn_few_kernel<T, D, false>, grid, dim3(kKdWarps * 32), smem, st, p));
     MSB_LAUNCH_CHECK("kv8_attn");
   }
   if (pl.splits > 1) {
@@ -487,7 +557,7 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   p.scale = scale; p.heads = heads; p.G = heads / p.c.heads; p.window = window; p.chunk = pl.chunk; p.splits = pl.splits;
   p.tile = pl.rows; p.step = pl.step;
   p.q_vec = qv; p.out_vec = ov; p.status = tb.status;
-#define KV8_GO(T) return c->head_dim == 64 ? launch_attn<T, 64>(p, pl, elem_type, st, dev) : launch_attn<T, 128>(p, pl, elem_type, st, dev)
+#define KV8_GO(T) return c->head_dim == 64 ? launch_attn<T, 64>(p, pl, elem_type, st, dev, sms) : launch_attn<T, 128>(p, pl, elem_type, st, dev, sms)
   if (elem_type == F32) KV8_GO(float);
   if (elem_type == F16) KV8_GO(__half);
   KV8_GO(__nv_bfloat16);

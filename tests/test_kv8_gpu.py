@@ -279,6 +279,24 @@ def test_attention_over_blocks_of_very_different_scales(dt, dim):
         check_attn(c, q, out, out, dim ** -0.5, 0, None)
 
 
+@pytest.mark.parametrize("seqs,kv_heads,G", [([(1, 1000), (1, 3)], 2, 8), ([(1, 260)], 8, 8), ([(3, 900), (0, 700), (2, 129), (1, 1)], 1, 20),
+                                             ([(4, 1024)], 4, 4), ([(1, 128), (1, 129), (1, 640)], 3, 1)])
+@pytest.mark.parametrize("dt", ("f32", "bf16"))
+@pytest.mark.parametrize("dim", (64, 128))
+def test_attention_whose_parts_are_a_cluster(seqs, kv_heads, G, dim, dt):
+    """Few rows over a few hundred keys: parts without keys among them, and rows that are not there."""
+    from macseek_b200 import kv8
+    c = R.Case(seqs, kv_heads, dim, 32, seed=G, pad=1)
+    cache, batch, e = c.cache(), c.batch(), enc()
+    for window, sink in ((0, True), (100, False), (300, True)):
+        q = c.randn(c.rows, kv_heads * G, dim, dt=dt, mul=3.0)
+        out = torch.full_like(q, 7)
+        sinks = c.randn(kv_heads * G) if sink else None
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, kv_heads * G), window=window, sinks=sinks)
+        e.wait()
+        check_attn(c, q, out, torch.full_like(q, 7), dim ** -0.5, window, sinks)
+
+
 def test_attention_results_do_not_depend_on_the_run_or_on_neighbours():
     from macseek_b200 import kv8
     c = R.Case([(1, 900), (1, 3000), (2, 64)], 2, 128, 64, seed=5)
