@@ -265,6 +265,65 @@ inline void encode_sparse(Enc& e, DecodeCaches& s, const Buffer& q, const Buffer
                           n_win, s.ckv.ptr(), (const int*)s.topk_list.ptr(), s.topk, s.heads, s.D, (float*)out.ptr(),
                           s.sparse_scratch.ptr(), s.sparse_scratch.size, e.stream), "encode_sparse");
 }
+// ---- grouped-query heads over an 8-bit cache (not in the reference, whose attention has one K == V row per token)
+struct Kv8Cache {         // codes [n_blocks][kv_heads][block][head_dim], scales f32 [n_blocks][kv_heads]
+  int n_blocks = 0, kv_heads = 8, head_dim = 128, block = 64;
+  Buffer k, v, k_scale, v_scale;
+  size_t code_bytes() const { return (size_t)n_blocks * kv_heads * block * head_dim; }
+  size_t scale_bytes() const { return (size_t)n_blocks * kv_heads * 4; }
+  msb_kv8_cache c() const {
+    return msb_kv8_cache{n_blocks, kv_heads, head_dim, block, k.ptr(), v.ptr(), (float*)k_scale.ptr(), (float*)v_scale.ptr()};
+  }
+};
+struct Kv8Batch {         // seq_start int32 [n_seq + 1], kv_len int32 [n_seq], table int32 [n_seq][table_stride]
+  int n_seq = 1, n_tokens = 1, max_new = 1, max_len = 1, table_stride = 1;
+  Buffer seq_start, kv_len, table;
+  msb_kv8_batch c() const {
+    return msb_kv8_batch{n_seq, n_tokens, max_new, max_len, (const int*)seq_start.ptr(), (const int*)kv_len.ptr(), (const int*)table.ptr(), table_stride};
+  }
+};
+struct HeadNormRope {     // rows of elem_type: q [n][heads][dim], k [n][kv_heads][dim], strides in elements (0: dense)
+  int elem_type = MSB_F32, heads = 64, kv_heads = 8, dim = 128, n_tokens = 1, n_pos = 1, rot = 64, first = 64;
+  bool halves = false;
+  float eps = 1e-6f;
+  int64_t q_stride = 0, k_stride = 0, q_out_stride = 0, k_out_stride = 0;
+  Buffer q, k, q_w, k_w, cs, pos, q_out, k_out;
+};
+inline void encode_head_norm_rope(Enc& e, const HeadNormRope& a) {
+  const int64_t qs = (int64_t)a.heads * a.dim, ks = (int64_t)a.kv_heads * a.dim;
+  check(msb_head_norm_rope(a.elem_type, a.q.ptr(), a.heads, a.q_stride ? a.q_stride : qs, (const float*)a.q_w.ptr(), a.k.ptr(), a.kv_heads,
+                           a.k_stride ? a.k_stride : ks, (const float*)a.k_w.ptr(), a.n_tokens, a.dim, a.eps, (const float*)a.cs.ptr(),
+                           (const int*)a.pos.ptr(), a.n_pos, a.rot, a.first, a.halves ? 1 : 0, a.q_out.ptr(), a.q_out_stride ? a.q_out_stride : qs,
+                           a.k_out.ptr(), a.k_out_stride ? a.k_out_stride : ks, e.stream), "encode_head_norm_rope");
+}
+inline void encode_kv8_write(Enc& e, const Kv8Cache& cache, const Kv8Batch& batch, int elem_type, const Buffer& k, const Buffer& v,
+                             int64_t k_stride = 0, int64_t v_stride = 0) {
+  const msb_kv8_cache c = cache.c();
+  const msb_kv8_batch b = batch.c();
+  const int64_t dense = (int64_t)cache.kv_heads * cache.head_dim;
+  check(msb_kv8_write(&c, &b, elem_type, k.ptr(), v.ptr(), k_stride ? k_stride : dense, v_stride ? v_stride : dense, e.stream), "encode_kv8_write");
+}
+inline void encode_kv8_read(Enc& e, const Kv8Cache& cache, const Kv8Batch& batch, int elem_type, const Buffer& k, const Buffer& v,
+                            int64_t k_stride = 0, int64_t v_stride = 0) {
+  const msb_kv8_cache c = cache.c();
+  const msb_kv8_batch b = batch.c();
+  const int64_t dense = (int64_t)cache.kv_heads * cache.head_dim;
+  check(msb_kv8_read(&c, &b, elem_type, k.ptr(), v.ptr(), k_stride ? k_stride : dense, v_stride ? v_stride : dense, e.stream), "encode_kv8_read");
+}
+inline size_t kv8_attn_scratch_bytes(const Kv8Cache& cache, const Kv8Batch& batch, int heads) {
+  const msb_kv8_cache c = cache.c();
+  const msb_kv8_batch b = batch.c();
+  return msb_kv8_attn_scratch_bytes(&c, &b, heads);
+}
+inline void encode_kv8_attn(Enc& e, const Kv8Cache& cache, const Kv8Batch& batch, int elem_type, const Buffer& q, int heads, float scale,
+                            const Buffer& out, const Buffer& scratch, int window = 0, const Buffer& sinks = Buffer(), int64_t q_stride = 0,
+                            int64_t out_stride = 0) {
+  const msb_kv8_cache c = cache.c();
+  const msb_kv8_batch b = batch.c();
+  const int64_t dense = (int64_t)heads * cache.head_dim;
+  check(msb_kv8_attn(&c, &b, elem_type, q.ptr(), q_stride ? q_stride : dense, heads, scale, window, (const float*)sinks.ptr(), out.ptr(),
+                     out_stride ? out_stride : dense, scratch.ptr(), scratch.size, e.stream), "encode_kv8_attn");
+}
 }  // namespace attn
 
 }  // namespace ms

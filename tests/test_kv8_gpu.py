@@ -434,3 +434,163 @@ def test_attention_of_what_is_not_a_number_ends():
         bad = (out.double() - ref).abs() > tol
         bad[0, :3] = False
         assert not bad.any()
+
+
+# ------------------------------------------------------------------------------------------------ as they are used
+class Model:
+    """The attention of one layer as an engine runs it: head norms and rotation, the cache, attention; and the same in 64 bits on what the
+    cache holds."""
+
+    def __init__(self, heads, kv_heads, dim, block, dt, seqs, blocks_each, seed=0):
+        from macseek_b200 import kv8
+        self.heads, self.kv_heads, self.dim, self.block, self.dt = heads, kv_heads, dim, block, R.DT[dt]
+        self.g = torch.Generator().manual_seed(seed)
+        self.cache = kv8.Cache(seqs * blocks_each + 1, kv_heads, dim, block)
+        self.table_host = (torch.randperm(seqs * blocks_each, generator=self.g) + 1).reshape(seqs, blocks_each)
+        self.table = self.table_host.int().cuda()
+        self.qw, self.kw = ((1 + 0.2 * torch.randn(dim, generator=self.g)).cuda() for _ in range(2))
+        ang = torch.arange(4096, dtype=torch.float64)[:, None] * torch.pow(1e4, -torch.arange(dim // 2) * 2 / dim)[None]
+        self.cs = torch.stack([ang.cos(), ang.sin()], -1).float().contiguous().cuda()
+
+    def step(self, e, x, pos, start, length, max_new, max_len, scratch=None, out=None, window=0):
+        """x: fused rows [n][(heads + 2 kv_heads) dim]; everything enqueued on e."""
+        from macseek_b200 import attn, kv8
+        n = x.shape[0]
+        q, k, v = (x[:, a * self.dim:b * self.dim].unflatten(1, (-1, self.dim)) for a, b in (
+            (0, self.heads), (self.heads, self.heads + self.kv_heads), (self.heads + self.kv_heads, self.heads + 2 * self.kv_heads)))
+        attn.encode_head_norm_rope(e, q, k, self.qw, self.kw, 1e-6, self.cs, pos, q, k, halves=True)
+        batch = kv8.Batch(start, length, self.table, n, max_new, max_len)
+        kv8.encode_kv8_write(e, self.cache, batch, k, v)
+        out = torch.empty(n, self.heads, self.dim, dtype=x.dtype, device="cuda") if out is None else out
+        kv8.encode_kv8_attn(e, self.cache, batch, q, out, kv8.attn_scratch(self.cache, batch, self.heads) if scratch is None else scratch, window=window)
+        return q, out
+
+    def check(self, q, out, seqs, window=0):
+        c = R.Case.__new__(R.Case)
+        c.seqs, c.kv_heads, c.dim, c.block, c.table_host = seqs, self.kv_heads, self.dim, self.block, self.table_host
+        c.k, c.v, c.ks, c.vs = self.cache.k, self.cache.v, self.cache.k_scale, self.cache.v_scale
+        c.start_host = [0]
+        for n, _ in seqs:
+            c.start_host.append(c.start_host[-1] + n)
+        ref, tol = R.attn_ref(c, q, out, self.dim ** -0.5, window)
+        assert ((out.double() - ref).abs() <= tol).all()
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dt,window", (("f32", 0), ("bf16", 0), ("bf16", 100)))
+def test_prompts_then_tokens(dt, window):
+    """Prompts of several lengths, a chunk behind one of them, then tokens one by one across the ends of blocks."""
+    m = Model(8, 2, 64, 32, dt, seqs=3, blocks_each=12)
+    e = enc()
+    lens = [0, 0, 0]
+    for new in ([200, 1, 63], [30, 17, 1], *([[1, 1, 1]] * 5), [1, 4, 2]):
+        start = [0]
+        for s, n in enumerate(new):
+            start.append(start[-1] + n)
+            lens[s] += n
+        x = torch.randn(start[-1], 12 * 64, generator=m.g).to(R.DT[dt]).cuda()
+        pos = i32(sum(([lens[s] - n + i for i in range(n)] for s, n in enumerate(new)), []))
+        was = x.clone()
+        q, out = m.step(e, x, pos, i32(start), i32(lens), max(new), max(lens), window=window)
+        e.wait()
+        m.check(q, out, list(zip(new, lens)), window)
+        # the rows that were written are the cache's, rounded to its format: half a step of the value or of the scale's smallest
+        for s, n in enumerate(new):
+            for which, rows in (("k", x[:, 8 * 64:10 * 64]), ("v", was[:, 10 * 64:])):
+                c = R.Case.__new__(R.Case)
+                c.seqs, c.block, c.table_host = list(zip(new, lens)), 32, m.table_host
+                c.k, c.v, c.ks, c.vs = m.cache.k, m.cache.v, m.cache.k_scale, m.cache.v_scale
+                held = c.held(s, which, lens[s] - n).transpose(0, 1)
+                want = rows[start[s]:start[s + 1]].unflatten(1, (2, 64)).double()
+                assert ((held - want).abs() <= want.abs() * 2.0 ** -4 + float(c.ks.max()) * 2.0 ** -9).all()
+
+
+def test_captured_steps_follow_their_arrays():
+    """A captured token step replayed as the sequences grow, its lengths and positions changed between replays."""
+    m = Model(16, 2, 128, 64, "bf16", seqs=4, blocks_each=8, seed=3)
+    e0 = enc()
+    lens = [1, 63, 64, 200]
+    x = torch.randn(sum(lens), 20 * 128, generator=m.g).bfloat16().cuda()
+    start = [0, 1, 64, 128, 328]
+    m.step(e0, x, i32([p for n in lens for p in range(n)]), i32(start), i32(lens), 200, 200)
+    e0.wait()
+    x, pos, start, length = torch.zeros(4, 20 * 128, dtype=torch.bfloat16, device="cuda"), i32([0] * 4), i32([0, 1, 2, 3, 4]), i32(lens)
+    from macseek_b200 import kv8
+    scratch = kv8.attn_scratch(m.cache, kv8.Batch(start, length, m.table, 4, 1, 512), 16)
+    out = torch.zeros(4, 16, 128, dtype=torch.bfloat16, device="cuda")
+    keep = (m.cache.k.clone(), m.cache.v.clone(), m.cache.k_scale.clone(), m.cache.v_scale.clone())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        m.step(enc(s), x, pos, start, length, 1, 512, scratch, out)      # once before, as any program does
+    s.synchronize()
+    for a, b in zip((m.cache.k, m.cache.v, m.cache.k_scale, m.cache.v_scale), keep):
+        a.copy_(b)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        q, _ = m.step(enc(torch.cuda.current_stream()), x, pos, start, length, 1, 512, scratch, out)
+    for t in range(70):
+        lens = [n + 1 for n in lens]
+        x.copy_(torch.randn(4, 20 * 128, generator=m.g).bfloat16())
+        pos.copy_(i32([n - 1 for n in lens]))
+        length.copy_(i32(lens))
+        graph.replay()
+        if t % 10 == 0 or t > 66:
+            torch.cuda.synchronize()
+            m.check(q, out, [(1, n) for n in lens])
+    enc().wait()
+
+
+def test_calls_on_two_streams_at_once():
+    from macseek_b200 import kv8
+    cases = [R.Case([(1, 3000), (2, 800)], 2, 128, 64, seed=1), R.Case([(300, 700)], 2, 64, 16, seed=2), R.Case([(1, 900)], 4, 64, 32, seed=3)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    work = []
+    for c, s in zip(cases, streams):
+        q = c.randn(c.rows, c.kv_heads * 4, c.dim, dt="bf16")
+        work.append((c, s, q, torch.zeros_like(q), c.cache(), c.batch()))
+    scratch = [kv8.attn_scratch(w[4], w[5], w[2].shape[1]) for w in work]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (c, s, q, out, cache, batch), sc in zip(work, scratch):
+            kv8.encode_kv8_attn(enc(s), cache, batch, q, out, sc)
+    torch.cuda.synchronize()
+    for c, s, q, out, *_ in work:
+        check_attn(c, q, out, torch.zeros_like(out), c.dim ** -0.5, 0, None)
+
+
+def test_blocks_beyond_32_bits():
+    """A cache of over 4 GiB of codes: the last blocks, written, read and attended to by both kernels."""
+    from macseek_b200 import kv8
+    n, heads, dim, block = 70000, 8, 128, 64
+    k, v = (torch.empty(n, heads, block, dim, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = torch.ones(n, heads, device="cuda"), torch.ones(n, heads, device="cuda")
+    assert k.numel() > 2 ** 32
+    cache = kv8.Cache.of(k, v, ks, vs)
+    g = torch.Generator().manual_seed(1)
+    e = enc()
+    c = R.Case.__new__(R.Case)
+    c.kv_heads, c.dim, c.block, c.device, c.g = heads, dim, block, "cuda", g
+    c.table_host = torch.tensor([[n - 1, 3, n - 2, n - 7]])
+    c.k, c.v, c.ks, c.vs, c.start_host = k, v, ks, vs, [0, 200]
+    table = c.table_host.int().cuda()
+    rows = [c.randn(200, heads, dim, dt="bf16") for _ in range(2)]
+    batch = kv8.Batch(i32([0, 200]), i32([200]), table, 200, 200, 200)
+    kv8.encode_kv8_write(e, cache, batch, *rows)
+    back = [torch.empty_like(r) for r in rows]
+    kv8.encode_kv8_read(e, cache, batch, *back)
+    e.wait()
+    for a, b in zip(rows, back):
+        assert ((a.double() - b.double()).abs() <= a.double().abs() * 2.0 ** -4 + 2.0 ** -15).all()
+    for new in (1, 200):
+        c.seqs, c.start_host = [(new, 200)], [0, new]
+        batch = kv8.Batch(i32([0, new]), i32([200]), table, new, new, 200)
+        q = c.randn(new, 64, dim, dt="bf16", mul=2.0)
+        out = torch.zeros_like(q)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 64))
+        e.wait()
+        check_attn(c, q, out, out, dim ** -0.5, 0, None)
