@@ -152,9 +152,12 @@ def encode_head_norm_rope(e: Enc, q, k, q_w, k_w, eps, cs, pos, q_out, k_out, ro
     [rot_first, rot_first + 2 cs.shape[1]) by position pos [n] (int32; negative: a padding row, left out) in one pass, into
     q_out, k_out (may be q, k).  cs: F32 [positions][pairs][2] as make_rope_table's; pairs are neighbouring dims, or with
     halves dims half the rotated width apart.  (No counterpart in the reference: encode_kv_window has one head.)"""
-    dev = cs.device
-    rc = kv8._call(e, dev, _lib.host().msb_host_head_norm_rope, q, k, q_w, k_w, eps, cs, pos, q_out, k_out, dev.index, rot_first, int(halves),
-                   _NORM_ROPE)
+    dev, st = cs.device, e.stream
+    i = dev.index
+    if st.device_index == i == torch.cuda.current_device():
+        rc = _lib.host().msb_host_head_norm_rope(q, k, q_w, k_w, eps, cs, pos, q_out, k_out, i, rot_first, halves, _NORM_ROPE, st.cuda_stream)
+    else:
+        rc = kv8._elsewhere(e, dev, _lib.host().msb_host_head_norm_rope, q, k, q_w, k_w, eps, cs, pos, q_out, k_out, i, rot_first, halves, _NORM_ROPE)
     if rc > 0:                     # not plainly right: say why
         x = k if q is None else q
         kv8._want(x is not None and x.dim() == 3, "head_norm_rope: q or k must be [n][heads][D]")

@@ -8,7 +8,8 @@ class Enc:
     until the enqueued work is done and raises if a kernel reported a device-side failure."""
 
     def __init__(self, stream=None):
-        self.stream = stream if stream is not None else torch.cuda.current_stream()
+        # (the device as a number: looking it up again costs more than the rest)
+        self.stream = stream if stream is not None else torch.cuda.current_stream(torch.cuda.current_device())
 
     @property
     def handle(self):

@@ -85,6 +85,10 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   __shared__ float s_m[kKdWarps][kKdRows], s_l[kKdWarps][kKdRows], s_bm[kKdRows], s_bl[kKdRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int tiles = gridDim.y / p.c.heads, kvh = blockIdx.y / tiles, m0 = (blockIdx.y % tiles) * kKdRows;
+  // without a window the keys of this part are known before the sequence is: its first blocks' ids are asked for at the same time
+  const int* table = p.b.table + (size_t)blockIdx.z * p.b.table_stride;
+  const int early = (blockIdx.x * p.chunk + kKdStep * (warp + kKdWarps * (lane >> 1)) + 16 * (lane & 1)) >> p.c.shift;
+  const int early_id = early < p.b.table_stride ? __ldg(table + early) : -1;
   const Kv8Seq sq = kv8_seq(p.b, blockIdx.z, p.status);
   const int R = sq.n * p.G;
   if (m0 >= R) return;
@@ -94,7 +98,6 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
   if (!CLUSTER && k0 >= k1) return;
   const int steps = k1 > k0 ? (k1 - k0 + kKdStep - 1) / kKdStep : 0;
   const int mine = steps > warp ? (steps - warp + kKdWarps - 1) / kKdWarps : 0;
-  const int* table = p.b.table + (size_t)blockIdx.z * p.b.table_stride;
 
   // ---- block ids and scales of the warp's next 16 steps, half a step (16 tokens: one block) per lane; ve = -inf: no such block
   int ids = -1;
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv
     const int key = k0 + kKdStep * (warp + kKdWarps * (i + (lane >> 1))) + 16 * (lane & 1);
     ids = -1; ksc = 0.f; vex = -INFINITY;
     if (key < k1) {
-      ids = __ldg(table + (key >> p.c.shift));
+      ids = i == 0 && kr.lo == 0 ? early_id : __ldg(table + (key >> p.c.shift));
       if (ids < 0 || ids >= p.c.n_blocks) { ids = -1; atomicCAS(p.status, 0, kDevBadBatch); }
       else {
         ksc = __ldg(p.c.ks + (size_t)ids * p.c.heads + kvh);

@@ -16,15 +16,15 @@ def _want(ok, what):
         raise _lib.MsbError(what)
 
 
-def _call(e, device, fn, *args):
-    """fn(*args) with `device` current (the library works on the current device), which has to be the stream's too."""
-    st = e.stream
-    if st.device_index != device.index:
-        raise _lib.MsbError("tensors on %s, the stream on %s" % (device, st.device))
-    if torch.cuda.current_device() == device.index:
-        return fn(*args, st.cuda_stream)
+_current = torch.cuda.current_device
+
+
+def _elsewhere(e, device, fn, *args):
+    """fn(*args, stream) on a device that is not the current one (the library works on the current device); it has to be the stream's."""
+    if e.stream.device_index != device.index:
+        raise _lib.MsbError("tensors on %s, the stream on %s" % (device, e.stream.device))
     with torch.cuda.device(device):
-        return fn(*args, st.cuda_stream)
+        return fn(*args, e.stream.cuda_stream)
 
 
 class Cache:
@@ -43,7 +43,7 @@ class Cache:
         return c
 
     def _set(self, k, v, k_scale, v_scale):
-        self.device = k.device
+        self.device, self.index = k.device, k.device.index
         for name, t, dt, shape in (("k", k, torch.uint8, k.shape), ("v", v, torch.uint8, k.shape),
                                    ("k_scale", k_scale, torch.float32, k.shape[:2]), ("v_scale", v_scale, torch.float32, k.shape[:2])):
             _want(t.is_cuda and t.device == self.device, "kv8 cache: %s must be on one CUDA device" % name)
@@ -62,7 +62,7 @@ class Batch:
 
     def __init__(self, seq_start, kv_len, table, n_tokens, max_new, max_len):
         n = kv_len.shape[0]
-        self.device = kv_len.device
+        self.device, self.index = kv_len.device, kv_len.device.index
         for name, t, shape in (("seq_start", seq_start, (n + 1,)), ("kv_len", kv_len, (n,)), ("table", table, (n, table.shape[-1]))):
             _want(t.is_cuda and t.device == self.device, "kv8 batch: %s must be on one CUDA device" % name)
             _want(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(),
@@ -92,8 +92,13 @@ _WRITE, _READ, _ATTN = (_lib.address(f) for f in (_lib.lib.msb_kv8_write, _lib.l
 
 
 def _kv(e, cache, batch, k, v, call, what):
-    dev = cache.device
-    rc = _call(e, dev, _lib.host().msb_host_kv8_rows, k, v, cache.addr, batch.addr, dev.index, call) if batch.device == dev else 1
+    i, st, dev = cache.index, e.stream, cache.device
+    if batch.index != i:
+        rc = 1
+    elif st.device_index == i == _current():
+        rc = _lib.host().msb_host_kv8_rows(k, v, cache.addr, batch.addr, i, call, st.cuda_stream)
+    else:
+        rc = _elsewhere(e, dev, _lib.host().msb_host_kv8_rows, k, v, cache.addr, batch.addr, i, call)
     if rc > 0:                     # not plainly right: say why
         _want(batch.device == dev, "%s: cache and batch on different devices" % what)
         ty = _rows("k", k, batch.n_tokens, cache.kv_heads, cache.head_dim, dev)
@@ -123,9 +128,15 @@ def attn_scratch(cache: Cache, batch: Batch, heads):
 def encode_kv8_attn(e: Enc, cache: Cache, batch: Batch, q, out, scratch, scale=None, window=0, sinks=None):
     """Attention of the rows q [n_tokens][heads][head_dim] over the cache, which holds their tokens already, into out
     (scale: head_dim^-0.5 if None; window 0: everything up to the row's own token; sinks: F32 [heads] or None)."""
-    dev = cache.device
-    rc = _call(e, dev, _lib.host().msb_host_kv8_attn, q, out, scratch, sinks, cache.addr, batch.addr, dev.index,
-               cache.head_dim ** -0.5 if scale is None else scale, window, _ATTN) if batch.device == dev else 1
+    i, st, dev = cache.index, e.stream, cache.device
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    if batch.index != i:
+        rc = 1
+    elif st.device_index == i == _current():
+        rc = _lib.host().msb_host_kv8_attn(q, out, scratch, sinks, cache.addr, batch.addr, i, scale, window, _ATTN, st.cuda_stream)
+    else:
+        rc = _elsewhere(e, dev, _lib.host().msb_host_kv8_attn, q, out, scratch, sinks, cache.addr, batch.addr, i, scale, window, _ATTN)
     if rc > 0:                     # not plainly right: say why
         _want(batch.device == dev and scratch.device == dev, "kv8_attn: cache, batch and scratch on different devices")
         heads = q.shape[1] if q.dim() == 3 else 0

@@ -205,7 +205,7 @@ def test_mirror_refuses_another_device_than_the_streams():
     from macseek_b200 import _lib, kv8
     e = type("E", (), {"stream": _Stream()})()
     with pytest.raises(_lib.MsbError, match="stream"):
-        kv8._call(e, torch.device("cuda", 0), None)
+        kv8._elsewhere(e, torch.device("cuda", 0), None)
 
 
 @pytest.mark.parametrize("shape,stride,ok", [((3, 2, 64), (128, 64, 1), True), ((3, 2, 64), (400, 64, 1), True), ((1, 2, 64), (9, 64, 1), True),
