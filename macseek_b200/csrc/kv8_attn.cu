@@ -73,9 +73,12 @@ __device__ __forceinline__ float4 kd_load4_of(uint32_t addr) {
   return v;
 }
 
+// Blocks of an SM: F32 rows of 128 dims need more registers than a third of an SM's threads have (64 ragged sequences: 147 us with two blocks,
+// 211 with three and 270 bytes a thread in local memory).  Four of 64 dims gain nothing (200K tokens, bf16: 44 us with three).
+constexpr int kd_blocks(bool f32, int dim) { return f32 && dim == 128 ? 2 : 3; }
 // CLUSTER: the parts of a row are the blocks of a cluster, which join them through one another's shared memory
 template <class T, int D, bool CLUSTER>
-__global__ void __launch_bounds__(kKdWarps * 32, 3) kv8_attn_few_kernel(const Kv8AttnParams p) {
+__global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) kv8_attn_few_kernel(const Kv8AttnParams p) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr bool TWO = sizeof(T) == 4;
@@ -513,7 +516,7 @@ static int launch_attn(const Kv8AttnParams& p, const Kv8Plan& pl, int elem_type,
       done[dev & 63] = true;
     }
     const dim3 grid(pl.splits, p.c.heads * pl.tiles, p.b.n_seq);
-    // few parts of few rows: one launch, the parts a cluster (a token of 64 heads over 8 behind 998: 10.5 -> KD_US us).  Not once the blocks do
+    // few parts of few rows: one launch, the parts a cluster (a token of 64 heads over 8 behind 998: F32: 11.2 us with a second launch, 8.1).  Not once the blocks do
     // not all run at once: those of short sequences would wait for the long ones of their cluster
     if (pl.splits > 1 && pl.splits <= kKdCluster && (int64_t)grid.x * grid.y * grid.z <= 2 * sms) {
       MSB_CUDA(launch_clusters(kv8_attn_few_kernel<T, D, true>, grid, dim3(kKdWarps * 32), pl.splits, smem, st, p));

@@ -1,6 +1,7 @@
 // Index arithmetic of the 8-bit cache's kernels as plain C++, for the kernels and for tests on the host: which rows, blocks and keys a
 // block of threads works on, for any contents of a batch's device arrays.  Nothing here gives an index outside what the arguments allow.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 
 #ifdef __CUDACC__
@@ -97,16 +98,16 @@ inline Kv8Plan kv8_plan(int n_seq, int max_new, int max_len, int kv_heads, int h
     Kv8Plan& pl = plans[k];
     const int span = kv8_span(max_len, pl.rows, G, window, pl.step), unit = k ? pl.step : 64, top = k ? most.many : most.few;
     pl.tiles = (int)up(rows, pl.rows);
-    const int64_t units = pl.tiles * groups;
-    // few: keys of 16 rows that an SM does in a us, by three blocks (one alone: 1 / 1.7 of them); many: us a key of a block's rows
-    const double speed = f32 ? (dim == 64 ? 182 : 81) : (dim == 64 ? 230 : 155), per_key = f32 ? (dim == 64 ? 0.032 : 0.044) : (dim == 64 ? 0.031 : 0.034);
+    const int64_t units = pl.tiles * groups, room = k ? 1 : f32 && dim == 128 ? 2 : 3;      // blocks an SM at once
+    // few: keys of 16 rows that an SM does in a us, by all its blocks (one alone: 1 / 1.7 of them); many: us a key of a block's rows
+    const double speed = f32 ? (dim == 64 ? 182 : 115) : (dim == 64 ? 230 : 155), per_key = f32 ? (dim == 64 ? 0.032 : 0.044) : (dim == 64 ? 0.031 : 0.034);
     for (int n = 1, last = 0; n <= top; n++) {
       const int chunk = kv8_max((int)(up(up(span, n), unit) * unit), kKv8Least), parts = (int)up(span, chunk);
       if (parts == last) continue;
       last = parts;
-      const int64_t blocks = (int64_t)(units * parts * part) + 1, at_once = blocks > 2 * sms ? 3 : blocks > sms ? 2 : 1;
+      const int64_t blocks = (int64_t)(units * parts * part) + 1, at_once = std::min(room, up(blocks, sms));
       const double one = k ? 7 + per_key * chunk : 2 + chunk * (at_once > 1 ? at_once : 1.7) / speed;
-      const double us = 4 + (double)up(blocks, k ? sms : 3 * sms) * one + (parts > 1 ? 3 + joined * parts : 0);
+      const double us = 4 + (double)up(blocks, room * sms) * one + (parts > 1 ? 3 + joined * parts : 0);
       if (pl.splits == 0 || us < best[k]) { best[k] = us; pl.chunk = chunk; pl.splits = parts; }
     }
   }
