@@ -2,8 +2,9 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w ;  (a, b) -> (a c - b s, a s + b c) for the pairs of dims [first, first + rot)
 // Each value is read and written once.  Eight elements per lane, so a head of 64 / 128 / 256 dims is 8 / 16 / 32 lanes and a warp has
 // 4 / 2 / 1 heads at a time; the gains are multiplied into the token's (cos, sin) factors, which stay in a lane's registers for all its
-// heads.  A block is one warp with all heads of a token: what a token costs before its first head is then spread over all of them
-// (4096 tokens with 64 + 8 heads of 128, bf16: 38.6 us = 3.97 TB/s, bound by issue and by the latency of each group of loads).
+// heads, and four groups of heads are on the way while four are computed: a warp's chain of loads is what bounds it (4096 tokens with 64 + 8
+// heads of 128, bf16: 58 us with a block a token, 40.3 with a warp a token, 33.5 = 4.57 TB/s with the next loads ahead; neither eight groups
+// nor more warps an SM with fewer registers end sooner).
 #include <algorithm>
 #include "kv8.cuh"
 
@@ -20,29 +21,30 @@ struct NormRopeParams {
   NormRopeSide q, k;
   const float* cs;
   const int* pos;
-  int D, rot, first, halves, n_pos, per_block, cs_vec, w_vec;
+  int n_tokens, D, rot, first, halves, n_pos, per_block, cs_vec, w_vec;
   float eps;
   int* status;
 };
 
-constexpr int kNrThreads = 32;      // (of 64: 40.0 us, of 128: 49.1 for the prompt above; a chunk of 999 tokens 5.8 and 7.8)
+constexpr int kNrWarps = 4;      // tokens of a block
 
 // LANES lanes a head (a power of two >= D / 8)
 template <class T, int LANES>
-__global__ void __launch_bounds__(kNrThreads) head_norm_rope_kernel(const NormRopeParams p) {
+__global__ void __launch_bounds__(32 * kNrWarps) head_norm_rope_kernel(const NormRopeParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kGroups = kNrThreads / LANES, kWarp = 32 / LANES;      // heads of a block, of a warp
+  constexpr int kGroups = 32 / LANES;                     // heads of a warp
   typedef typename Elems<T>::Raw Raw;
   constexpr int kHeads = 4;                               // heads of a group of lanes that are under way at a time
-  const int lane = threadIdx.x & 31, l = threadIdx.x % LANES, group = threadIdx.x / LANES, warp0 = group / kWarp * kWarp;
-  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x, l = lane % LANES, group = lane / LANES;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= p.n_tokens) return;
   const int d = 8 * l;
   const bool live = d < p.D;
   const int pos = __ldg(p.pos + row);
   if (pos < 0) return;                                    // a padding row
   if (pos >= p.n_pos) {
-    if (threadIdx.x == 0) atomicCAS(p.status, 0, kDevBadBatch);
+    if (lane == 0) atomicCAS(p.status, 0, kDevBadBatch);
     return;
   }
   const bool turned = live && d >= p.first && d < p.first + p.rot;
@@ -99,15 +101,19 @@ __global__ void __launch_bounds__(kNrThreads) head_norm_rope_kernel(const NormRo
     uint64_t a2[4], b2[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) { a2[i] = kv8_two(a[2 * i], a[2 * i + 1]); b2[i] = kv8_two(b[2 * i], b[2 * i + 1]); }
-    for (int hb = h0 + group; hb - group + warp0 < h1;) { // whole warps: the shuffles need every lane
+    for (int hb = h0 + group; hb - group < h1; hb += kHeads * kGroups) {     // whole warps: the shuffles need every lane
+      Raw now[kHeads];
+#pragma unroll
+      for (int i = 0; i < kHeads; i++) now[i] = raw[i];
+      if (hb - group + kHeads * kGroups < h1) load(hb + kHeads * kGroups);   // on the way while these are computed
 #pragma unroll
       for (int i = 0; i < kHeads; i++) {
         const int h = hb + i * kGroups;
-        if (h - group + warp0 >= h1) break;               // none of the warp's
+        if (h - group >= h1) break;               // none of the warp's
         float v[8], o[8];
-        Elems<T>::open(raw[i], v);
+        Elems<T>::open(now[i], v);
         if (p.halves) {
-          Elems<T>::open(Elems<T>::from_lane(raw[i], partner), o);
+          Elems<T>::open(Elems<T>::from_lane(now[i], partner), o);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; j++) o[j] = turned ? v[j ^ 1] : v[j];
@@ -130,19 +136,20 @@ __global__ void __launch_bounds__(kNrThreads) head_norm_rope_kernel(const NormRo
           kv8_apart(kv8_mul2(r2, kv8_fma2(x2[j], a2[j], kv8_mul2(kv8_two(o[2 * j], o[2 * j + 1]), b2[j]))), v[2 * j], v[2 * j + 1]);
         if (live && h < h1) Elems<T>::store(y + h * p.D, vec, v);
       }
-      hb += kHeads * kGroups;
-      if (hb - group + warp0 < h1) load(hb);
     }
   }
 }
 
 template <class T>
 static int launch_norm_rope(NormRopeParams& p, int n_tokens, cudaStream_t st) {
-  const int lanes = p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, groups = kNrThreads / lanes;
-  // all heads in a block once the tokens alone fill the GPU twice, a head a group of lanes before
-  p.per_block = n_tokens >= 2 * 148 ? p.q.heads + p.k.heads : groups;
-  const dim3 grid((unsigned)n_tokens, (unsigned)((p.q.heads + p.k.heads + p.per_block - 1) / p.per_block));
-  auto go = [&](auto kern) { return launch_pdl(kern, grid, dim3(kNrThreads), 0, st, p); };
+  const int lanes = p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32, groups = 32 / lanes, heads = p.q.heads + p.k.heads;
+  // all heads of a token in a warp once the tokens alone fill the GPU twice; before, a head a group of lanes
+  const bool many = n_tokens >= 2 * 148;
+  p.per_block = many ? heads : groups;
+  p.n_tokens = n_tokens;
+  const int warps = many ? kNrWarps : 1;
+  const dim3 grid((unsigned)((n_tokens + warps - 1) / warps), (unsigned)((heads + p.per_block - 1) / p.per_block)), block(32, warps);
+  auto go = [&](auto kern) { return launch_pdl(kern, grid, block, 0, st, p); };
   MSB_CUDA(lanes == 8 ? go(head_norm_rope_kernel<T, 8>) : lanes == 16 ? go(head_norm_rope_kernel<T, 16>) : go(head_norm_rope_kernel<T, 32>));
   MSB_LAUNCH_CHECK("head_norm_rope");
   return kOk;

@@ -53,14 +53,16 @@ struct Kv8RowsParams {
 };
 
 constexpr int kKv8Threads = 256;
+constexpr int kv8_block_threads(int group) { return group > kKv8Threads ? group : kKv8Threads; }
 
-// THREADS threads a work item (32 or 256), each with up to MOST pieces of eight values of a unit
+// THREADS threads a unit (whole warps), each with up to MOST pieces of eight values
 template <class T, int D, int THREADS, int MOST>
-__global__ void __launch_bounds__(kKv8Threads) kv8_write_kernel(const Kv8RowsParams p) {
+__global__ void __launch_bounds__(kv8_block_threads(THREADS)) kv8_write_kernel(const Kv8RowsParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kGroups = kKv8Threads / THREADS, kRow = D / 8, kWarps = THREADS / 32;
-  __shared__ float s_max[2][kWarps];
+  constexpr int kGroups = kv8_block_threads(THREADS) / THREADS, kRow = D / 8, kWarps = THREADS / 32;
+  __shared__ float s_top[kGroups][2][kWarps];
+  float (&s_max)[2][kWarps] = s_top[threadIdx.x / THREADS];
   const int tid = threadIdx.x % THREADS, sh = p.c.shift, units = 2 * p.c.heads, step = gridDim.y * kGroups;
   int s;
   const Kv8Item it = kv8_item(p.b, sh, p.each, blockIdx.x, p.status, s);
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_write_kernel(const Kv8RowsPar
     top = warp_max(top);
     if (THREADS > 32) {
       if ((tid & 31) == 0) s_max[turn][tid >> 5] = top;
-      __syncthreads();                                              // (also: every thread has read the scale that is written below)
+      bar_sync_named(1 + threadIdx.x / THREADS, THREADS);           // (also: every thread has read the scale that is written below)
 #pragma unroll
       for (int i = 0; i < kWarps; i++) top = fmaxf(top, s_max[turn][i]);
     }
@@ -231,21 +233,27 @@ static int launch_rows(bool write, Kv8RowsParams& p, cudaStream_t st) {
   const int64_t each = kv8_touched(p.b.max_new, sh), all = kv8_items(p.b.n_tokens, p.b.n_seq, sh);
   const int64_t items = std::min(each * p.b.n_seq, all);
   p.each = each * p.b.n_seq <= all ? (int)each : 0;
-  // a warp a unit while its new rows are few; for more a block, which goes over the units of a block while there are blocks enough
-  // (reading 16 sequences of up to 8192 tokens: 90.5 us with 4 or 8 blocks an SM, 84.7 with 16, 82.7 with 32, 87.3 with 64)
   if (items > 0x7fffffff) return fail(kErrLimit, "kv8: too many rows");
-  const bool few = (int64_t)std::min(p.b.max_new, 1 << sh) * (D / 8) <= 64;
-  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(units, items * units / (148 * (write ? 8 : 32))));
-  const dim3 grid((unsigned)items, write && few ? (units + 7) / 8 : (units + per - 1) / per);
-  auto go = [&](auto kern) { return launch_pdl(kern, grid, dim3(kKv8Threads), 0, st, p); };
+  // blocks of threads of `group` threads a unit, each over `per` units while there are blocks enough for every SM
+  auto go = [&](auto kern, int group, int64_t an_sm) {
+    const int groups = kv8_block_threads(group) / group, per = (int)std::max<int64_t>(1, std::min<int64_t>(units, items * units / (148 * an_sm * groups)));
+    return launch_pdl(kern, dim3((unsigned)items, (units + per * groups - 1) / (per * groups)), dim3(kv8_block_threads(group)), 0, st, p);
+  };
+  const int pieces = (D / 8) << sh;
   if (!write) {
-    const int pieces = (D * (int)sizeof(T) / 16) << sh;
-    MSB_CUDA(pieces <= 4 * kKv8Threads ? go(kv8_read_kernel<T, D, 4>) : pieces <= 8 * kKv8Threads ? go(kv8_read_kernel<T, D, 8>)
-                                                                                                   : go(kv8_read_kernel<T, D, 16>));
+    // (16 sequences of up to 8192 tokens: 90.5 us with 4 or 8 blocks an SM, 84.7 with 16, 82.7 with 32, 87.3 with 64)
+    const int steps = (D * (int)sizeof(T) / 16) << sh;
+    MSB_CUDA(steps <= 4 * kKv8Threads ? go(kv8_read_kernel<T, D, 4>, 256, 32) : steps <= 8 * kKv8Threads ? go(kv8_read_kernel<T, D, 8>, 256, 32)
+                                                                                                         : go(kv8_read_kernel<T, D, 16>, 256, 32));
+  } else if ((int64_t)std::min(p.b.max_new, 1 << sh) * (D / 8) <= 64) {
+    MSB_CUDA(go(kv8_write_kernel<T, D, 32, 2>, 32, 1 << 20));       // few new rows: a warp a unit
+  } else {
+    // four pieces a thread, whatever the block (ragged prompts, bf16, blocks of 16 / 64 / 128 tokens: 19.7 / 17.8 / 23.5 us; with 256 threads
+    // for all of them 31.3 / 17.3 / 31.2)
+    MSB_CUDA(pieces <= 128 ? go(kv8_write_kernel<T, D, 32, 4>, 32, 4) : pieces <= 256 ? go(kv8_write_kernel<T, D, 64, 4>, 64, 4)
+             : pieces <= 512 ? go(kv8_write_kernel<T, D, 128, 4>, 128, 4) : pieces <= 1024 ? go(kv8_write_kernel<T, D, 256, 4>, 256, 4)
+                                                                                   : go(kv8_write_kernel<T, D, 512, 4>, 512, 4));
   }
-  else if (few) MSB_CUDA(go(kv8_write_kernel<T, D, 32, 2>));
-  else if ((D / 8) << sh <= 4 * kKv8Threads) MSB_CUDA(go(kv8_write_kernel<T, D, 256, 4>));
-  else MSB_CUDA(go(kv8_write_kernel<T, D, 256, 8>));
   MSB_LAUNCH_CHECK(write ? "kv8_write" : "kv8_read");
   return kOk;
 }
