@@ -168,13 +168,13 @@ __global__ void __launch_bounds__(kv8_block_threads(THREADS)) kv8_write_kernel(c
   }
 }
 
-// 16 bytes of a row a thread and step: eight values, four of F32; up to MOST steps a unit
-template <class T, int D, int MOST>
+// 16 bytes of a row a thread and step: eight values, four of F32; THREADS threads a unit, up to MOST steps
+template <class T, int D, int THREADS, int MOST>
 __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8RowsParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int V = 16 / sizeof(T), kRow = D / V;
-  const int sh = p.c.shift, units = 2 * p.c.heads;
+  constexpr int V = 16 / sizeof(T), kRow = D / V, kGroups = kKv8Threads / THREADS;
+  const int sh = p.c.shift, units = 2 * p.c.heads, tid = threadIdx.x % THREADS, step = gridDim.y * kGroups;
   int s;
   const Kv8Item it = kv8_item(p.b, sh, p.each, blockIdx.x, p.status, s);
   if (it.n == 0) return;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8RowsPara
     const uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D + it.at * D;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-      const int c = threadIdx.x + i * kKv8Threads;
+      const int c = tid + i * THREADS;
       if (c < pieces) {
         if (V == 8) {
           const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes) + c);
@@ -199,21 +199,21 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8RowsPara
     }
     next_scale = __ldg(((u & 1) ? p.c.vs : p.c.ks) + head);
   };
-  int u = blockIdx.y;
+  int u = blockIdx.y * kGroups + threadIdx.x / THREADS;
   if (u < units) load(u);
-  for (; u < units; u += gridDim.y) {
+  for (; u < units; u += step) {
 #pragma unroll
     for (int i = 0; i < MOST; i++)
 #pragma unroll
       for (int j = 0; j < V / 4; j++) w[i][j] = next[i][j];
     scale = next_scale;
-    if (u + gridDim.y < units) load(u + gridDim.y);
+    if (u + step < units) load(u + step);
     const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
     const int64_t stride = values ? p.v_stride : p.k_stride;
     T* rows = static_cast<T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-      const int c = threadIdx.x + i * kKv8Threads;
+      const int c = tid + i * THREADS;
       if (c >= pieces) break;
       float o[V];
 #pragma unroll
@@ -241,10 +241,12 @@ static int launch_rows(bool write, Kv8RowsParams& p, cudaStream_t st) {
   };
   const int pieces = (D / 8) << sh;
   if (!write) {
-    // (16 sequences of up to 8192 tokens: 90.5 us with 4 or 8 blocks an SM, 84.7 with 16, 82.7 with 32, 87.3 with 64)
+    // (16 sequences of up to 8192 tokens, blocks of 64: 90.5 us with 4 or 8 blocks an SM, 84.7 with 16, 82.6 with 32, 87.3 with 64; blocks of
+    // 16 tokens with 256 threads for all: 124)
     const int steps = (D * (int)sizeof(T) / 16) << sh;
-    MSB_CUDA(steps <= 4 * kKv8Threads ? go(kv8_read_kernel<T, D, 4>, 256, 32) : steps <= 8 * kKv8Threads ? go(kv8_read_kernel<T, D, 8>, 256, 32)
-                                                                                                         : go(kv8_read_kernel<T, D, 16>, 256, 32));
+    MSB_CUDA(steps <= 128 ? go(kv8_read_kernel<T, D, 32, 4>, 32, 32) : steps <= 256 ? go(kv8_read_kernel<T, D, 64, 4>, 64, 32)
+             : steps <= 512 ? go(kv8_read_kernel<T, D, 128, 4>, 128, 32) : steps <= 1024 ? go(kv8_read_kernel<T, D, 256, 4>, 256, 32)
+             : steps <= 2048 ? go(kv8_read_kernel<T, D, 256, 8>, 256, 32) : go(kv8_read_kernel<T, D, 256, 16>, 256, 32));
   } else if ((int64_t)std::min(p.b.max_new, 1 << sh) * (D / 8) <= 64) {
     MSB_CUDA(go(kv8_write_kernel<T, D, 32, 2>, 32, 1 << 20));       // few new rows: a warp a unit
   } else {
