@@ -159,7 +159,7 @@ int head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, 
                    int64_t k_stride, const float* k_w, int n_tokens, int D, float eps, const float* cs, const int* pos, int n_pos, int rot,
                    int first, int halves, void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride, cudaStream_t st) {
   const char* what = "head_norm_rope";
-  if (n_tokens <= 0 || q_heads < 0 || k_heads < 0 || q_heads + k_heads <= 0 || q_heads > 65535 || k_heads > 65535)
+  if (n_tokens <= 0 || q_heads < 0 || k_heads < 0 || q_heads + k_heads <= 0 || q_heads > 32767 || k_heads > 32767)
     return fail(kErrArg, "%s: %d rows of %d + %d heads", what, n_tokens, q_heads, k_heads);
   if (D < 8 || D > 256 || D % 8) return fail(kErrArg, "%s: head dim %d (multiples of 8 up to 256)", what, D);
   if (rot < 0 || rot % 2 || first < 0 || first + rot > D || first % 8 || rot % (halves ? 16 : 8))

@@ -552,7 +552,7 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   MSB_CUDA(cudaGetDevice(&dev));
   if ((rc = kv8_sms(&sms))) return rc;
   const Kv8Plan pl = kv8_plan(p.b.n_seq, p.b.max_new, p.b.max_len, p.c.heads, heads, c->head_dim, elem_type == F32, window, sms);
-  if (pl.many ? pl.tiles > 65535 : (int64_t)p.c.heads * pl.tiles > 65535) return fail(kErrLimit, "%s: too many rows", what);
+  if (pl.many && pl.tiles > 65535) return fail(kErrLimit, "%s: too many rows", what);
   if ((int64_t)p.b.n_tokens * heads > 0x7fffffff) return fail(kErrLimit, "%s: too many rows", what);
   const size_t need = kv8_part_bytes(p.b, heads, c->head_dim, pl.splits);
   if (need && (!scratch || scratch_bytes < need)) return fail(kErrScratch, "%s: scratch too small (%zu < %zu)", what, scratch_bytes, need);

@@ -101,7 +101,7 @@ inline Kv8Plan kv8_plan(int n_seq, int max_new, int max_len, int kv_heads, int h
     const int64_t units = pl.tiles * groups, room = k ? 1 : f32 && dim == 128 ? 2 : 3;      // blocks an SM at once
     // few: keys of 16 rows that an SM does in a us, by all its blocks (one alone: 1 / 1.7 of them); many: us a key of a block's rows
     const double speed = f32 ? (dim == 64 ? 182 : 115) : (dim == 64 ? 230 : 155), per_key = f32 ? (dim == 64 ? 0.032 : 0.044) : (dim == 64 ? 0.031 : 0.034);
-    for (int n = 1, last = 0; n <= top; n++) {
+    for (int n = 1, last = 0; n <= top; n = n < top ? kv8_min(top, n + kv8_max(1, n / 8)) : top + 1) {
       const int chunk = kv8_max((int)(up(up(span, n), unit) * unit), kKv8Least), parts = (int)up(span, chunk);
       if (parts == last) continue;
       last = parts;
@@ -111,7 +111,7 @@ inline Kv8Plan kv8_plan(int n_seq, int max_new, int max_len, int kv_heads, int h
       if (pl.splits == 0 || us < best[k]) { best[k] = us; pl.chunk = chunk; pl.splits = parts; }
     }
   }
-  return best[0] <= best[1] ? plans[0] : plans[1];
+  return best[0] <= best[1] && (int64_t)plans[0].tiles * kv_heads <= 65535 ? plans[0] : plans[1];     // (of a grid's second dimension)
 }
 
 }  // namespace msb

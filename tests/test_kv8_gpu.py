@@ -389,6 +389,21 @@ def test_refusals_that_need_a_device():
         kv8.encode_kv8_attn(e, cache, batch, q.cpu(), torch.empty_like(q), kv8.attn_scratch(cache, batch, 16))
     with pytest.raises(_lib.MsbError):
         kv8.attn_scratch(cache, batch, 15)
+    with pytest.raises((_lib.MsbError, RuntimeError)):               # no strides to ask for: refused, not ended
+        kv8.encode_kv8_attn(e, cache, batch, q.to_sparse(), torch.empty_like(q), kv8.attn_scratch(cache, batch, 16))
+    with pytest.raises(_lib.MsbError):
+        kv8.encode_kv8_write(e, cache, batch, c.randn(c.rows, 2, 128), c.randn(c.rows, 2, 128).half())
+    with pytest.raises(_lib.MsbError):
+        kv8.encode_kv8_read(e, cache, batch, c.randn(c.rows, 2, 64), c.randn(c.rows, 2, 128))
+    with pytest.raises(_lib.MsbError, match="sinks"):
+        kv8.encode_kv8_attn(e, cache, batch, q, torch.empty_like(q), kv8.attn_scratch(cache, batch, 16), sinks=torch.zeros(15, device="cuda"))
+    from macseek_b200 import attn
+    cs, pos = torch.zeros(9, 32, 2, device="cuda"), torch.zeros(c.rows, dtype=torch.int32, device="cuda")
+    for bad in (dict(q=q.cpu()), dict(q_w=torch.ones(64, device="cuda")), dict(pos=pos.long()), dict(cs=cs[:, :, 0]), dict(q_out=q.half())):
+        a = dict(q=q, q_w=None, pos=pos, cs=cs, q_out=torch.empty_like(q))
+        a.update(bad)
+        with pytest.raises(_lib.MsbError):
+            attn.encode_head_norm_rope(e, a["q"], None, a["q_w"], None, 1e-6, a["cs"], a["pos"], a["q_out"], None)
     e.wait()
 
 

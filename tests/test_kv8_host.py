@@ -116,7 +116,7 @@ def test_attention_takes_the_kernel_and_the_split_that_end_sooner(tmp_path):
     cases = {(1, 1, 1, 8, 64, 128, 0, 0): (0, 1), (1, 1, 999, 8, 64, 128, 1, 0): (0, 8), (1, 1, 200000, 8, 64, 128, 0, 0): (0, 55),
              (64, 1, 8192, 8, 64, 128, 0, 0): (0, 4), (64, 1, 8192, 8, 64, 128, 0, 128): (0, 1), (16, 4, 4004, 8, 64, 64, 0, 0): (0, 5),
              (1, 64, 64, 8, 64, 64, 0, 0): (0, 1), (1, 4096, 4096, 8, 64, 128, 0, 0): (1, 1), (1, 4096, 4096, 8, 64, 128, 1, 0): (1, 1),
-             (5, 333, 8525, 4, 32, 64, 0, 4096): (1, 1), (1, 256, 1256, 8, 64, 128, 0, 0): (1, 2), (1, 16, 16016, 8, 64, 128, 1, 0): (1, 18)}
+             (5, 333, 8525, 4, 32, 64, 0, 4096): (1, 1), (1, 256, 1256, 8, 64, 128, 0, 0): (1, 2), (1, 300000, 300000, 8, 64, 64, 0, 16): (1, 1), (1, 16, 16016, 8, 64, 128, 1, 0): (1, 18)}
     src, exe = tmp_path / "t.cpp", tmp_path / "t"
     src.write_text('#include "kv8_index.h"\n#include <cstdio>\nint main() {\n' + "\n".join(
         '{ auto p = msb::kv8_plan(%s, 148); printf("%%d %%d\\n", p.many, p.splits); }' % ", ".join(map(str, c)) for c in cases) + "\n}\n")
@@ -181,7 +181,7 @@ def test_head_norm_rope_refuses():
            ko=BASE, kos=128):
         return _lib.lib.msb_head_norm_rope(ty, q, qh, qs, None, k, kh, ks, None, n, D, 1e-6, cs, pos, n_pos, rot, first, halves, qo, qos, ko, kos, None)
     assert go(ty=2) == -2
-    for kw in (dict(q=None), dict(k=None), dict(qo=None), dict(ko=None), dict(qs=255), dict(kos=127), dict(n=0), dict(qh=0, kh=0), dict(qh=-1),
+    for kw in (dict(q=None), dict(k=None), dict(qo=None), dict(ko=None), dict(qs=255), dict(kos=127), dict(n=0), dict(qh=0, kh=0), dict(qh=-1), dict(kh=32768, ks=1 << 40, kos=1 << 40),
                dict(D=60), dict(D=264), dict(D=0), dict(rot=62), dict(rot=72), dict(rot=-8), dict(first=8), dict(first=-8, rot=32), dict(first=4, rot=32),
                dict(rot=8, halves=1), dict(rot=56, halves=1), dict(pos=None), dict(cs=None), dict(n_pos=0), dict(q=BASE + 2), dict(ty=1, ko=BASE + 1)):
         assert go(**kw) == -1, kw
