@@ -8,7 +8,9 @@
 //   S         has two buffers a row tile: the scores of a tile are there before the weights of the one before are done.  (One buffer of 128
 //             keys reads the queries half as often: 375 us for the prompt below, but 107 for the chunks.)
 //   F32 rows  queries and weights are two halves each: one row tile, and twice the products
-//   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32), O from 128 on; F32: [256, 320) the second halves of P
+//   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32), O from 128 on; F32: [256, 320) the second halves of P, whose
+//             products have a sum of their own from 384 on.  (The tensor core cuts off what a sum does not hold: F32 scores begin with the
+//             queries' second halves, and the long sums over keys take no more steps than 16-bit rows' do.)
 // Bound by the exponentials (16 a clock beside those on the multiply-add pipe) and by shared memory: the products read 48 KB a tile and row
 // tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 403 us = 683 TFLOP/s, of which a sixth goes into a block's
 // start and end; ragged chunks of up to 333 tokens, 32 heads over 4 of 64, behind up to 8192: 98 us.  Every wait is bounded.
@@ -27,7 +29,7 @@ struct KmShape {
   static constexpr int kSoft = 4 * kTiles, kMma = kSoft + 4, kWarps = kMma + 1;
   static constexpr int kQ = kKmRows * D * 2, kKv = kKmKeys * D * 2;      // bytes of a row tile's queries (a term), of a tile's keys or values
   static constexpr int kSmem = 4096 + kTiles * kTerms * kQ + 2 * kKmStages * kKv;
-  static constexpr uint32_t kO = 128, kLow = 256;
+  static constexpr uint32_t kO = 128, kLow = 256, kO2 = 384;       // (kO2: what the second halves of the weights add to O)
 };
 struct KmHead {
   uint64_t kfull[kKmStages], kempty[kKmStages], vfull[kKmStages], vempty[kKmStages];
@@ -147,11 +149,11 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
 #pragma unroll 1
           for (int t = 0; t < nt; t++) {
 #pragma unroll
-            for (int e = 0; e < S::kTerms; e++)
+            for (int e = S::kTerms - 1; e >= 0; e--)
 #pragma unroll
               for (int k = 0; k < D / 16; k++)
                 km_mma_ss(tmem + t * 256 + b * kKmKeys, q_d + (uint32_t)((t * S::kTerms + e) * (S::kQ >> 4) + (k >> 2) * (16384 >> 4) + (k & 3) * 2),
-                          k_d + (uint32_t)(s * (S::kKv >> 4) + (k >> 2) * (kKmKeys * 128 >> 4) + (k & 3) * 2), is, (e | k) ? 1u : 0u);
+                          k_d + (uint32_t)(s * (S::kKv >> 4) + (k >> 2) * (kKmKeys * 128 >> 4) + (k & 3) * 2), is, (e < S::kTerms - 1 || k) ? 1u : 0u);
             ts_commit(&hd->sfull[t][b]);
           }
           ts_commit(&hd->kempty[s]);
@@ -171,8 +173,8 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           for (int e = 0; e < S::kTerms; e++)
 #pragma unroll
             for (int k = 0; k < kKmKeys / 16; k++)
-              ts_mma_f16(tmem + t * 256 + S::kO, tmem + (e ? S::kLow + b * 32 : t * 256 + b * kKmKeys) + k * 8,
-                         v_d + (uint32_t)(s * (S::kKv >> 4) + k * (2048 >> 4)), io, (j | e | k) ? 1u : 0u);
+              ts_mma_f16(tmem + (e ? S::kO2 : t * 256 + S::kO), tmem + (e ? S::kLow + b * 32 : t * 256 + b * kKmKeys) + k * 8,
+                         v_d + (uint32_t)(s * (S::kKv >> 4) + k * (2048 >> 4)), io, (j | k) ? 1u : 0u);
           ts_commit(j + 1 < n ? &hd->odone[t] : &hd->ofull[t]);
         }
         __syncwarp();
@@ -456,12 +458,13 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           __syncwarp();
           ts_fence_after();
 #pragma unroll 1
-          for (int k = 0; k < D / 16; k++) {
-            ts_ld16(to + 16 * k, w[0]);
+          for (int k = 0; k < S::kTerms * (D / 16); k++) {
+            const uint32_t at = k < D / 16 ? to + 16 * k : tmem + lanes + S::kO2 + 16 * (k - D / 16);
+            ts_ld16(at, w[0]);
             ts_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; i++) w[0][i] = __float_as_uint(__uint_as_float(w[0][i]) * f);
-            ts_st16(to + 16 * k, w[0]);
+            ts_st16(at, w[0]);
           }
           ts_wait_st();
         }
@@ -512,6 +515,13 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
         __syncwarp();
         ts_ld16(to + 16 * c, a);
         ts_wait_ld();
+        if (TWO) {
+          uint32_t b[16];
+          ts_ld16(tmem + lanes + S::kO2 + 16 * c, b);
+          ts_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i++) a[i] = __float_as_uint(__uint_as_float(a[i]) + __uint_as_float(b[i]));
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           float v[8];
