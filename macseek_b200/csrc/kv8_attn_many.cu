@@ -12,7 +12,7 @@
 //             products have a sum of their own from 384 on.  (The tensor core cuts off what a sum does not hold: F32 scores begin with the
 //             queries' second halves, and the long sums over keys take no more steps than 16-bit rows' do.)
 // Bound by the exponentials (16 a clock beside those on the multiply-add pipe) and by shared memory: the products read 48 KB a tile and row
-// tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 403 us = 683 TFLOP/s, of which a sixth goes into a block's
+// tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 403 us = 683 TFLOP/s, of which an eighth goes into a block's
 // start and end; ragged chunks of up to 333 tokens, 32 heads over 4 of 64, behind up to 8192: 98 us.  Every wait is bounded.
 #include <algorithm>
 #include "kv8_attn.cuh"
