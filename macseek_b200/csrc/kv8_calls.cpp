@@ -63,7 +63,7 @@ extern "C" int msb_host_kv8_attn(PyObject* q, PyObject* out, PyObject* scratch, 
     Rows x, y;
     void* s;
     const at::Tensor* w = tensor(scratch, device);
-    if (!w || !rows(q, device, x) || !rows(out, device, y) || !same(x, b->n_tokens, x.heads, c->head_dim, y.type) ||
+    if (!w || !w->is_contiguous() || !rows(q, device, x) || !rows(out, device, y) || !same(x, b->n_tokens, x.heads, c->head_dim, y.type) ||
         !same(y, x.n, x.heads, x.dim, x.type) || !vector(sinks, device, at::kFloat, x.heads, &s) || (s && THPVariable_Unpack(sinks).dim() != 1))
       return kNotTaken;
     return call(c, b, x.type, x.p, x.stride, (int)x.heads, (float)scale, window, static_cast<const float*>(s), y.p, y.stride, w->data_ptr(),

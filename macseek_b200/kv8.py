@@ -139,6 +139,7 @@ def encode_kv8_attn(e: Enc, cache: Cache, batch: Batch, q, out, scratch, scale=N
         rc = _elsewhere(e, dev, _lib.host().msb_host_kv8_attn, q, out, scratch, sinks, cache.addr, batch.addr, i, scale, window, _ATTN)
     if rc > 0:                     # not plainly right: say why
         _want(batch.device == dev and scratch.device == dev, "kv8_attn: cache, batch and scratch on different devices")
+        _want(scratch.is_contiguous(), "kv8_attn: scratch must be contiguous")
         heads = q.shape[1] if q.dim() == 3 else 0
         ty = _rows("q", q, batch.n_tokens, heads, cache.head_dim, dev)
         _want(_rows("out", out, batch.n_tokens, heads, cache.head_dim, dev) == ty, "q and out must be of one type")

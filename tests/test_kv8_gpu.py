@@ -407,6 +407,21 @@ def test_refusals_that_need_a_device():
     e.wait()
 
 
+def test_scratch_that_is_not_one_piece_of_memory_is_refused():
+    """Elements of an expanded or strided tensor are not the bytes behind its pointer."""
+    from macseek_b200 import _lib, kv8
+    c = R.Case([(1, 5000)], 2, 128, 64, seed=1)
+    cache, batch = c.cache(), c.batch()
+    q = c.randn(c.rows, 16, 128)
+    e, out = enc(), torch.empty_like(q)
+    whole = kv8.attn_scratch(cache, batch, 16)
+    for bad in (whole[:1].expand(whole.numel()), torch.empty(2 * whole.numel(), dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(_lib.MsbError, match="contiguous"):
+            kv8.encode_kv8_attn(e, cache, batch, q, out, bad)
+    kv8.encode_kv8_attn(e, cache, batch, q, out, whole)
+    e.wait()
+
+
 @pytest.mark.parametrize("dt", ("f32", "bf16"))
 @pytest.mark.parametrize("n", (1, 64))
 def test_attention_where_the_largest_logit_comes_late_or_is_huge(n, dt):
