@@ -152,6 +152,8 @@ def encode_head_norm_rope(e: Enc, q, k, q_w, k_w, eps, cs, pos, q_out, k_out, ro
     [rot_first, rot_first + 2 cs.shape[1]) by position pos [n] (int32; negative: a padding row, left out) in one pass, into
     q_out, k_out (may be q, k).  cs: F32 [positions][pairs][2] as make_rope_table's; pairs are neighbouring dims, or with
     halves dims half the rotated width apart.  (No counterpart in the reference: encode_kv_window has one head.)"""
+    if not 0 <= rot_first <= 0x7fffffff:
+        kv8._fits("head_norm_rope: rot_first", rot_first)
     dev, st = cs.device, e.stream
     i = dev.index
     if st.device_index == i == torch.cuda.current_device():

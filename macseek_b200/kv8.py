@@ -16,6 +16,13 @@ def _want(ok, what):
         raise _lib.MsbError(what)
 
 
+def _fits(what, *numbers):
+    """Numbers that the C calls take in 32 bits, not negative."""
+    for x in numbers:
+        if not 0 <= x <= 0x7fffffff:
+            raise _lib.MsbError("%s: %d is negative or does not fit 32 bits" % (what, x))
+
+
 _current = torch.cuda.current_device
 
 
@@ -62,6 +69,7 @@ class Batch:
 
     def __init__(self, seq_start, kv_len, table, n_tokens, max_new, max_len):
         n = kv_len.shape[0]
+        _fits("kv8 batch", n, n_tokens, max_new, max_len, table.shape[-1])
         self.device, self.index = kv_len.device, kv_len.device.index
         for name, t, shape in (("seq_start", seq_start, (n + 1,)), ("kv_len", kv_len, (n,)), ("table", table, (n, table.shape[-1]))):
             _want(t.is_cuda and t.device == self.device, "kv8 batch: %s must be on one CUDA device" % name)
@@ -119,6 +127,7 @@ def encode_kv8_read(e: Enc, cache: Cache, batch: Batch, k, v):
 
 def attn_scratch(cache: Cache, batch: Batch, heads):
     """Scratch of encode_kv8_attn for this cache and batch (any window); calls that overlap in time need one each."""
+    _fits("kv8: heads", heads)
     with torch.cuda.device(cache.device):
         n = _lib.lib.msb_kv8_attn_scratch_bytes(cache.ref, batch.ref, heads)
     _want(n > 0, "kv8: " + _lib.lib.msb_last_error().decode())
@@ -128,6 +137,8 @@ def attn_scratch(cache: Cache, batch: Batch, heads):
 def encode_kv8_attn(e: Enc, cache: Cache, batch: Batch, q, out, scratch, scale=None, window=0, sinks=None):
     """Attention of the rows q [n_tokens][heads][head_dim] over the cache, which holds their tokens already, into out
     (scale: head_dim^-0.5 if None; window 0: everything up to the row's own token; sinks: F32 [heads] or None)."""
+    if not 0 <= window <= 0x7fffffff:
+        _fits("kv8_attn: window", window)
     i, st, dev = cache.index, e.stream, cache.device
     if scale is None:
         scale = cache.head_dim ** -0.5

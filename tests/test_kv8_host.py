@@ -220,3 +220,21 @@ def test_mirror_takes_rows_with_dense_heads_only(shape, stride, ok):
     else:
         with pytest.raises(_lib.MsbError):
             kv8._rows("x", t, *want, t.device)
+
+
+def test_mirror_refuses_numbers_beyond_32_bits():
+    """Structures and arguments of the C calls are 32-bit: a larger number would arrive as another one."""
+    from macseek_b200 import _lib, attn, kv8
+    i32 = dict(dtype=torch.int32)
+    for bad in ((1 << 32) + 1, 1 << 31, -1):
+        for at in range(3):
+            sizes = [1, 1, 1]
+            sizes[at] = bad
+            with pytest.raises(_lib.MsbError, match="32 bits"):
+                kv8.Batch(torch.zeros(2, **i32), torch.zeros(1, **i32), torch.zeros(1, 1, **i32), *sizes)
+        with pytest.raises(_lib.MsbError, match="32 bits"):
+            kv8.attn_scratch(None, None, bad)
+        with pytest.raises(_lib.MsbError, match="32 bits"):
+            kv8.encode_kv8_attn(None, None, None, None, None, None, window=bad)
+        with pytest.raises(_lib.MsbError, match="32 bits"):
+            attn.encode_head_norm_rope(None, None, None, None, None, 1e-6, None, None, None, None, rot_first=bad)
