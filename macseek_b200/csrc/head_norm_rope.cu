@@ -162,7 +162,7 @@ int head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, 
   if (n_tokens <= 0 || q_heads < 0 || k_heads < 0 || q_heads + k_heads <= 0 || q_heads > 32767 || k_heads > 32767)
     return fail(kErrArg, "%s: %d rows of %d + %d heads", what, n_tokens, q_heads, k_heads);
   if (D < 8 || D > 256 || D % 8) return fail(kErrArg, "%s: head dim %d (multiples of 8 up to 256)", what, D);
-  if (rot < 0 || rot % 2 || first < 0 || first + rot > D || first % 8 || rot % (halves ? 16 : 8))
+  if (rot < 0 || rot % 2 || first < 0 || rot > D || first > D - rot || first % 8 || rot % (halves ? 16 : 8))
     return fail(kErrArg, "%s: rotation of %d dims from %d on (first a multiple of 8, the count of 8, by halves of 16)", what, rot, first);
   if (!pos || n_pos <= 0 || (rot && !cs)) return fail(kErrArg, "%s: null pointer or no positions", what);
   NormRopeParams p{};

@@ -85,7 +85,7 @@ extern "C" int msb_host_head_norm_rope(PyObject* q, PyObject* k, PyObject* q_w, 
     const at::Tensor* f = tensor(cs, device);
     if (a.n != b.n || a.dim != b.dim || a.type != b.type || !vector(q_w, device, at::kFloat, a.dim, &qw) || !vector(k_w, device, at::kFloat, a.dim, &kw) ||
         pos == Py_None || !vector(pos, device, at::kInt, a.n, &p) || !f || f->scalar_type() != at::kFloat || f->dim() != 3 || f->size(2) != 2 ||
-        !f->is_contiguous() || f->size(0) > 0x7fffffff || a.n > 0x7fffffff)
+        !f->is_contiguous() || f->size(0) > 0x7fffffff || f->size(1) > 0x3fffffff || a.n > 0x7fffffff)
       return kNotTaken;
     return call(a.type, a.p, (int)a.heads, a.stride, static_cast<const float*>(qw), b.p, (int)b.heads, b.stride, static_cast<const float*>(kw), (int)a.n,
                 (int)a.dim, (float)eps, static_cast<const float*>(f->data_ptr()), static_cast<const int*>(p), (int)f->size(0), (int)(2 * f->size(1)),

@@ -238,3 +238,11 @@ def test_mirror_refuses_numbers_beyond_32_bits():
             kv8.encode_kv8_attn(None, None, None, None, None, None, window=bad)
         with pytest.raises(_lib.MsbError, match="32 bits"):
             attn.encode_head_norm_rope(None, None, None, None, None, 1e-6, None, None, None, None, rot_first=bad)
+
+
+@pytest.mark.parametrize("rot,first", [(64, 2147483640), (8, 2147483640), (2147483640, 8), (2147483640, 2147483640)])
+def test_head_norm_rope_refuses_dims_whose_sum_passes_32_bits(rot, first):
+    from macseek_b200 import _lib
+    assert _lib.lib.msb_head_norm_rope(0, BASE, 4, 256, None, BASE, 2, 128, None, 3, 64, 1e-6, BASE, BASE, 9, rot, first, 0, BASE, 256, BASE, 128,
+                                       None) == -1
+    assert b"rotation" in _lib.lib.msb_last_error()
