@@ -427,10 +427,12 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
         }
         const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
         if (!__any_sync(0xffffffffu, most > 60000.f && !lost)) break;
-        // to the next power of two above the sum, or, where that is beyond 32 bits, to the largest exponent.  A row whose products are
-        // infinite has none, and beyond 2^35 exponents are too coarse for one: after four times its weights stay what they are
+        // to the next power of two above the sum, or, where that is beyond 32 bits or near the end of km_exp2_fma's range (which a sum then
+        // does not show to be passed), to the largest exponent.  A row whose products are infinite has none, and beyond 2^35 exponents are
+        // too coarse for one: after four times its weights stay what they are
+        constexpr float kFar = 100.f;
         float up = most > 60000.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) : 0.f;
-        if (__any_sync(0xffffffffu, up > 128.f)) {
+        if (__any_sync(0xffffffffu, up > kFar)) {
           float top = -INFINITY;
 #pragma unroll 1
           for (int k = 0; k < 4; k++) {
@@ -444,7 +446,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
             }
             __syncwarp();
           }
-          if (up > 128.f) {
+          if (up > kFar) {
             lost = !(top < INFINITY);
             up = lost ? 0.f : ceilf(top);
           }

@@ -1,0 +1,32 @@
+"""Attention over the 8-bit cache at the ends of what its kernels hold: keys far above the others."""
+import pytest
+import torch
+
+import kv8_ref as R
+from test_kv8_gpu import check_attn, enc
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("n,dim", ((1, 64), (600, 64), (600, 128)))
+def test_attention_where_one_key_is_far_above_the_others(n, dim, dt):
+    """One key, or two, about 100, 400, 600 or 5000 binary exponents above all before it, at each of 16 places of a tile that is not the first."""
+    from macseek_b200 import kv8
+    G, scale = 8, 2.0 ** -8
+    c = R.Case([(n, 1000)], 4, dim, 16, seed=3)
+    c.k.fill_(0)
+    c.ks.fill_(1)
+    blk = int(c.table_host[0, 20])
+    q = torch.zeros(c.rows, 4 * G, dim, dtype=R.DT[dt], device="cuda")
+    q[:, :, 5] = torch.tensor([100.0, 400.0, 600.0, 5000.0], device="cuda").repeat(8).to(R.DT[dt]) * 0.6875      # times ln 2, about
+    cache, batch, e = c.cache(), c.batch(), enc()
+    scratch = kv8.attn_scratch(cache, batch, 4 * G)
+    for places in [(p,) for p in range(16)] + [(6, 7), (14, 15), (0, 6)]:
+        c.k[blk] = 0
+        for p in places:
+            c.k[blk, :, p, 5] = 0x78                                 # 256
+        out = torch.zeros_like(q)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, scale=scale)
+        e.wait()
+        check_attn(c, q, out, torch.zeros_like(out), scale, 0, None)
