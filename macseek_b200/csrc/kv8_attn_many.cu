@@ -504,7 +504,8 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
       if (whole) {
         float sum = l;
         if (p.sinks) sum += km_exp2(p.sinks[head] * kLog2e - (m == -INFINITY ? 0.f : m));
-        mul = sum > 0.f ? 1.f / sum : sum != sum ? sum : 0.f;
+        // (a row that sees nothing has no reference, and a sum only of what km_exp2_fma makes of its -infinities)
+        mul = sum != sum ? sum : m > -INFINITY && sum > 0.f ? 1.f / sum : 0.f;
       } else if (live) {
         *reinterpret_cast<float2*>(kv8_part_ml(p, D) + 2 * at) = make_float2(m, l);
       }

@@ -30,3 +30,27 @@ def test_attention_where_one_key_is_far_above_the_others(n, dim, dt):
         kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, scale=scale)
         e.wait()
         check_attn(c, q, out, torch.zeros_like(out), scale, 0, None)
+
+
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+def test_rows_that_see_no_block_are_zero_beside_rows_that_do(dt):
+    """The first blocks of a prompt are not there: its first rows see nothing, whatever scale the later blocks' values have."""
+    from macseek_b200 import _lib, kv8
+    n, dim, gone = 1100, 64, 144              # (a tile of 256 rows is 32 tokens: 16 of them see nothing)
+    c = R.Case([(n, n)], 4, dim, 16, seed=8)
+    c.table[0, :gone // 16] = -1
+    cache, batch, e = c.cache(), c.batch(), enc()
+    for ex in (0, 5, 6, -20) if dt == "f16" else (0, 6, 14, 24, -30):
+        c.vs.fill_(2.0 ** ex)
+        q = c.randn(n, 32, dim, dt=dt, mul=0.1)
+        out = torch.full_like(q, 7)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 32))
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 4
+        assert (out[:gone] == 0).all()
+        k, v = c.held(0, "k", gone), c.held(0, "v", gone)
+        seen = torch.arange(gone, n, device="cuda")[None] <= torch.arange(gone, n, device="cuda")[:, None]
+        for h in (0, 13, 31):
+            w = torch.softmax((q[gone:, h].double() @ k[h // 8].T * dim ** -0.5).masked_fill(~seen, -torch.inf), 1)
+            # weights and the output rounded to 11 bits (bf16: the output to 8), all else far finer
+            assert ((w @ v[h // 8]) - out[gone:, h].double()).abs().max() <= v.abs().max() * (2.0 ** -11 + 2.0 ** -14 + R.half_step(R.DT[dt])[0])
