@@ -15,7 +15,8 @@ namespace msb {
 
 enum : int { kDevBadBatch = 4, kDevNan = 5 };    // more codes of the device failure word
 // Exponents of scales.  The attention's weights carry the value scales, so that a sum of weights spans their range as well: with 100 binades
-// a token whose weight falls below 32 bits' range is 2^-26 of the sum at most.
+// a token whose weight falls below 32 bits' range is 2^-26 of the sum at most.  (The products take weights as halves, which lose what lies 2^-32
+// (F32 rows of many, 2^-43; few rows 2^-36) below the row's largest, code for code.)
 constexpr int kKv8MinExp = -50, kKv8MaxExp = 50;
 
 struct Kv8Cache {

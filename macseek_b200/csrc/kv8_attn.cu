@@ -6,7 +6,9 @@
 //   scores   the contraction may run over the dims in any order: a lane takes 16 neighbouring bytes of "its" token as eight pairs and
 //            the query's registers are laid out alike; a pair of codes is one conversion to two halves (exact)
 //   output   the tokens are contracted: bytes of two neighbouring tokens are interleaved and converted; lane g holds dims [g D / 8, (g + 1) D / 8)
-//   weights  the reference of the exponents moves only when a weight would pass 2^8: the sums are rescaled a few times, not at every new maximum
+//   weights  the reference of the exponents moves only when a weight would pass 2^15 (a half ends at 2^16), and then so that it becomes 2^11: the
+//            sums are rescaled a few times, not at every new maximum.  A half holds nothing below 2^-25: what a warp's N keys lose beside the
+//            largest of them is N 2^-36 at most
 // The queries are scaled by a power of two to at most 2 in a row and used as halves; F32 ones, and their weights, as two halves each.
 #include <algorithm>
 #include "kv8_attn.cuh"
@@ -14,6 +16,7 @@
 namespace msb {
 
 constexpr int kKdCluster = 8;      // blocks of a cluster at most
+constexpr float kKdTop = 15.f, kKdFirst = 11.f;      // exponents of a weight: above which the reference moves, and then
 constexpr int kKdWarps = 4, kKdStages = 2, kKdStep = kKv8FewStep, kKdRows = kKv8FewRows;
 
 __device__ __forceinline__ void kd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -252,10 +255,10 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+    if (__any_sync(0xffffffffu, top[0] - m[0] > kKdTop || top[1] - m[1] > kKdTop)) {      // (-infinity twice: no)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float n = top[h] > m[h] + 8.f ? top[h] : m[h], f = n == -INFINITY ? 1.f : kd_exp2(m[h] - n);
+        const float n = top[h] - m[h] > kKdTop ? top[h] - (fabsf(top[h]) < 1e6f ? kKdFirst : 0.f) : m[h], f = n == -INFINITY ? 1.f : kd_exp2(m[h] - n);
         m[h] = n; l[h] *= f;
 #pragma unroll
         for (int k = 0; k < NT; k++) { o[k][2 * h] *= f; o[k][2 * h + 1] *= f; }

@@ -54,3 +54,48 @@ def test_rows_that_see_no_block_are_zero_beside_rows_that_do(dt):
             w = torch.softmax((q[gone:, h].double() @ k[h // 8].T * dim ** -0.5).masked_fill(~seen, -torch.inf), 1)
             # weights and the output rounded to 11 bits (bf16: the output to 8), all else far finer
             assert ((w @ v[h // 8]) - out[gone:, h].double()).abs().max() <= v.abs().max() * (2.0 ** -11 + 2.0 ** -14 + R.half_step(R.DT[dt])[0])
+
+
+def one_long_context(S, n, L, dt, kv=8, G=8, dim=128, block=64):
+    """S sequences of n new tokens over one context of L tokens that they share: keys 0 but for the first, values of one sign."""
+    from macseek_b200 import kv8
+    g = torch.Generator().manual_seed(3)
+    nb = -(-L // block)
+    cache = kv8.Cache(nb, kv, dim, block)
+    cache.v.copy_((torch.rand(cache.v.shape, generator=g) * 128 + 128).to(R.FP8).view(torch.uint8))
+    cache.v_scale.fill_(2.0 ** -8)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch = kv8.Batch(torch.arange(S + 1, **i32) * n, torch.full((S,), L, **i32), torch.arange(nb, **i32)[None].expand(S, -1).contiguous(), S * n, n, L)
+    cache.k[0, :, 0, 0], cache.v[0, :, 0] = 0x38, 0x58               # 1, 16
+    v = (R.values(cache.v) * 2.0 ** -8).transpose(0, 1).reshape(kv, -1, dim)[:, :L]
+    q = torch.zeros(S * n, kv * G, dim, dtype=R.DT[dt], device="cuda")
+    q[:, :, 0] = 1
+    return cache, batch, q, v
+
+
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("S,n", ((128, 1), (1, 512)))
+@pytest.mark.parametrize("gap", (12.0, 15.0, 16.0, 17.5))
+def test_attention_keeps_small_weights_beside_a_large_one(S, n, dt, gap):
+    """The first key's logit is `gap` above those of thousands of others, whose weights together are a share of the sum that the output shows.
+
+    All values have one sign, so that weights off by 2^-11 (F32: 2^-21) and 2^x by 2^-20, the largest's among them, count by the result; a logit is
+    off by gap 2^-21, which counts by the share; sums over L tokens, 16 at a time and F32 in two halves, are off by (L / 8 + 32) 2^-23 of themselves."""
+    from macseek_b200 import kv8
+    L = 8192
+    cache, batch, q, v = one_long_context(S, n, L, dt)
+    out, e = torch.zeros_like(q), enc()
+    kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 64), scale=gap)
+    e.wait()
+    pos = torch.arange(L - n, L, device="cuda")
+    small = float(torch.exp(torch.tensor(-gap, dtype=torch.float64)))
+    total = 1 + small * pos.double()[:, None]
+    half, tiny = R.half_step(q.dtype)
+    share = (total - 1) / total
+    weight = (2.0 ** -21 if dt == "f32" else 2.0 ** -11) + 2.0 ** -20
+    for h in range(64):
+        rest = v[h // 8, 1:].cumsum(0)[pos - 1]
+        ref = (v[h // 8, 0] + small * rest) / total                  # [n][dim]
+        tol = (weight + (L / 8 + 32) * 2.0 ** -23) * ref + share * gap * 2.0 ** -21
+        got = out.view(S, n, 64, 128)[:, :, h].double()
+        assert ((got - ref).abs() <= tol * (1 + half) + half * ref.abs() + tiny).all(), (h, float((got - ref).abs().max()), float(tol.max()))
