@@ -17,6 +17,7 @@ namespace msb {
 
 constexpr int kKdCluster = 8;      // blocks of a cluster at most
 constexpr float kKdTop = 15.f, kKdFirst = 11.f;      // exponents of a weight: above which the reference moves, and then
+constexpr int kKdFold = 16;         // steps of a warp after which F32 rows' sums begin anew
 constexpr int kKdWarps = 4, kKdStages = 2, kKdStep = kKv8FewStep, kKdRows = kKv8FewRows;
 
 __device__ __forceinline__ void kd_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
   for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   const uint8_t* own = kd_smem + warp * kWarpBytes;
+  float4* sums = reinterpret_cast<float4*>(kd_smem + kKdWarps * kWarpBytes) + warp * NT * 32 + lane;      // F32: this lane's share of what O held
   const uint8_t* kl = own + KdTile<D>::key(g, t);
   const uint8_t* vl[2] = {own + 2 * kHalf + KdTile<D>::val(2 * t, D == 128 ? g : g >> 1) + (D == 128 ? 0 : 8 * (g & 1)),
                           own + 2 * kHalf + KdTile<D>::val(2 * t + 1, D == 128 ? g : g >> 1) + (D == 128 ? 0 : 8 * (g & 1))};
@@ -202,6 +204,15 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
     if (i + 1 < mine && ((i + 1) & 15) == 0) look_up(i + 1);
     fetch(i + 1);
     if (i && (i & 15) == 0) { ks_cur = ksc; ve_cur = vex; }
+    if (TWO && i && i % kKdFold == 0) {       // the tensor core cuts off what its sums do not hold: they begin anew, and what they held is added up
+#pragma unroll
+      for (int k = 0; k < NT; k++) {
+        float4 a = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
+        if (i > kKdFold) { const float4 b = sums[32 * k]; a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+        sums[32 * k] = a;
+        o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+      }
+    }
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
     const uint32_t st = (i & 1) * kStage;
@@ -262,6 +273,12 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
         m[h] = n; l[h] *= f;
 #pragma unroll
         for (int k = 0; k < NT; k++) { o[k][2 * h] *= f; o[k][2 * h + 1] *= f; }
+        if (TWO && i >= kKdFold)
+#pragma unroll 1
+          for (int k = 0; k < NT; k++) {
+            float2* b = reinterpret_cast<float2*>(sums + 32 * k) + h;
+            *b = make_float2(b->x * f, b->y * f);
+          }
       }
     }
 #pragma unroll
@@ -313,6 +330,12 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
     __syncwarp();                              // every lane has read the buffer that the next fetch fills
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (TWO && mine > kKdFold)
+#pragma unroll
+    for (int k = 0; k < NT; k++) {
+      const float4 b = sums[32 * k];
+      o[k][0] += b.x; o[k][1] += b.y; o[k][2] += b.z; o[k][3] += b.w;
+    }
 
   // ---- the four warps' results joined
 #pragma unroll
@@ -489,8 +512,9 @@ static int kv8_heads_check(const msb_kv8_cache* c, int heads, const char* what) 
   if (heads <= 0 || heads > 65535 || heads % c->kv_heads) return fail(kErrArg, "%s: %d query heads over %d key heads", what, heads, c->kv_heads);
   return kOk;
 }
-static size_t kv8_part_bytes(const Kv8Batch& b, int heads, int D, int splits) {
-  return splits > 1 ? sizeof(float) * (size_t)splits * b.n_tokens * heads * (D + 2) : 0;
+// the parts with their references and sums, or, for one part whose sums are begun anew (kv8_attn_many), what they held
+static size_t kv8_part_bytes(const Kv8Batch& b, int heads, int D, int splits, bool folds) {
+  return splits > 1 ? sizeof(float) * (size_t)splits * b.n_tokens * heads * (D + 2) : folds ? sizeof(float) * (size_t)b.n_tokens * heads * D : 0;
 }
 size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, int heads) {      // for rows of any type
   Kv8Cache cc; Kv8Batch bb;
@@ -502,7 +526,7 @@ size_t kv8_attn_scratch_bytes(const msb_kv8_cache* c, const msb_kv8_batch* b, in
     const Kv8Most m = kv8_most(bb.n_seq, bb.max_new, bb.max_len, cc.heads, heads, f32, sms);
     most = std::max(most, std::max(m.few, m.many));
   }
-  return 16 + kv8_part_bytes(bb, heads, c->head_dim, most);
+  return 16 + kv8_part_bytes(bb, heads, c->head_dim, most, bb.max_len > kKv8Fold);
 }
 
 template <class T, int D>
@@ -511,7 +535,8 @@ static int launch_attn(const Kv8AttnParams& p, const Kv8Plan& pl, int elem_type,
     const int rc = kv8_attn_many(p, pl.tiles, elem_type, D, st, dev);
     if (rc) return rc;
   } else {
-    const size_t smem = std::max<size_t>((size_t)kKdWarps * kKdStages * 2 * kKdStep * D, sizeof(float) * kKdWarps * kKdRows * (D + 4));
+    const size_t ring = (size_t)kKdWarps * kKdStages * 2 * kKdStep * D, sums = sizeof(T) == 4 ? sizeof(float) * kKdWarps * kKdRows * D : 0;
+    const size_t smem = std::max(ring + sums, sizeof(float) * kKdWarps * kKdRows * (D + 4));
     static bool done[64] = {};
     if (!done[dev & 63]) {
       MSB_CUDA(cudaFuncSetAttribute(kv8_attn_few_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -557,7 +582,7 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   const Kv8Plan pl = kv8_plan(p.b.n_seq, p.b.max_new, p.b.max_len, p.c.heads, heads, c->head_dim, elem_type == F32, window, sms);
   if (pl.many && pl.tiles > 65535) return fail(kErrLimit, "%s: too many rows", what);
   if ((int64_t)p.b.n_tokens * heads > 0x7fffffff) return fail(kErrLimit, "%s: too many rows", what);
-  const size_t need = kv8_part_bytes(p.b, heads, c->head_dim, pl.splits);
+  const size_t need = kv8_part_bytes(p.b, heads, c->head_dim, pl.splits, pl.many && elem_type != F32 && pl.chunk > kKv8Fold);
   if (need && (!scratch || scratch_bytes < need)) return fail(kErrScratch, "%s: scratch too small (%zu < %zu)", what, scratch_bytes, need);
   if (need && (reinterpret_cast<uintptr_t>(scratch) & 15)) return fail(kErrArg, "%s: scratch must be 16-byte aligned", what);
   Tables tb;

@@ -18,7 +18,7 @@ struct Kv8AttnParams {
   void* out;
   int64_t q_stride, out_stride;
   const float* sinks;
-  float* part;                 // [splits][n_tokens * heads][D], then [splits][n_tokens * heads] of (m, sum)
+  float* part;                 // [splits][n_tokens * heads][D], then [splits][n_tokens * heads] of (m, sum); one part: of its sums at most
   float scale;
   int heads, G, window;
   int chunk, splits, tile, step;   // keys of one split (a multiple of step), splits at most, rows of a tile, keys of a step

@@ -8,9 +8,11 @@
 //   S         has two buffers a row tile: the scores of a tile are there before the weights of the one before are done.  (One buffer of 128
 //             keys reads the queries half as often: 375 us for the prompt below, but 107 for the chunks.)
 //   F32 rows  queries and weights are two halves each: one row tile, and twice the products
-//   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32), O from 128 on; F32: [256, 320) the second halves of P, whose
-//             products have a sum of their own from 384 on.  (The tensor core cuts off what a sum does not hold: F32 scores begin with the
-//             queries' second halves, and the long sums over keys take no more steps than 16-bit rows' do.)
+//   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32, F32: its second halves in the others), O from 128 on; F32: the
+//             products of the second halves have a sum of their own from 384 on
+//   sums      the tensor core cuts off what a sum does not hold, so O is added to a sum elsewhere and begun anew every 512 keys (F32: tensor memory
+//             from 256 on) or 16384 (16 bits: the scratch), and F32 scores begin with the queries' second halves.  200K tokens with values
+//             of one sign, error without: 1.1e-3
 // Bound by the exponentials (16 a clock beside those on the multiply-add pipe) and by shared memory: the products read 48 KB a tile and row
 // tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 403 us = 683 TFLOP/s, of which an eighth goes into a block's
 // start and end; ragged chunks of up to 333 tokens, 32 heads over 4 of 64, behind up to 8192: 98 us.  Every wait is bounded.
@@ -21,7 +23,7 @@
 namespace msb {
 
 constexpr float kKmFirst = 7.f, kKmLow = 2048.f;      // exponent of the largest weight at first; what the second halves of weights are taken times
-constexpr int kKmKeys = kKv8ManyStep, kKmRows = 128, kKmStages = 4;
+constexpr int kKmKeys = kKv8ManyStep, kKmRows = 128, kKmStages = 4, kKmHeadBytes = 4096;
 
 template <class T, int D>
 struct KmShape {
@@ -29,8 +31,9 @@ struct KmShape {
   static constexpr int kTiles = kTwo ? 1 : 2, kTerms = kTwo ? 2 : 1;
   static constexpr int kSoft = 4 * kTiles, kMma = kSoft + 4, kWarps = kMma + 1;
   static constexpr int kQ = kKmRows * D * 2, kKv = kKmKeys * D * 2;      // bytes of a row tile's queries (a term), of a tile's keys or values
-  static constexpr int kSmem = 4096 + kTiles * kTerms * kQ + 2 * kKmStages * kKv;
-  static constexpr uint32_t kO = 128, kLow = 256, kO2 = 384;       // (kO2: what the second halves of the weights add to O, times kKmLow)
+  static constexpr int kSmem = 1024 + kKmHeadBytes + kTiles * kTerms * kQ + 2 * kKmStages * kKv;
+  static constexpr uint32_t kO = 128, kSum = 256, kO2 = 384;       // (kO2: what the second halves of the weights add to O, times kKmLow)
+  static constexpr int kFold = kTwo ? kKv8FoldF32 / kKmKeys : kKv8Fold / kKmKeys;      // tiles whose products the tensor core adds up
 };
 struct KmHead {
   uint64_t kfull[kKmStages], kempty[kKmStages], vfull[kKmStages], vempty[kKmStages];
@@ -38,9 +41,10 @@ struct KmHead {
   uint32_t tmem_base;
   int abort_flag;
   float f0[2 * kKmRows];
+  float2 kept[2 * kKmRows];                 // km_fold's
   float4 sc[kKmStages][kKmKeys / 16];       // key scale, exponent of the value scale, its inverse; of 16 tokens of a tile
 };
-static_assert(sizeof(KmHead) <= 3072, "the tiles follow");
+static_assert(sizeof(KmHead) <= kKmHeadBytes, "the tiles follow");
 
 // place of the 16 bytes `j` of row r, 64 halves a row: 8-row groups of 1024 bytes, 128-byte swizzle
 __device__ __forceinline__ uint32_t km_at(int r, int j) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((j ^ (r & 7)) << 4)); }
@@ -83,14 +87,58 @@ __device__ __forceinline__ void km_exp2_fma(float& a, float& b) {
   b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
 }
 
+// 16 numbers of what has been taken out of a row's O: tensor memory (F32), or the row's place of the scratch, where 16-bit rows' O leaves no room
+template <bool TWO>
+__device__ __forceinline__ void km_sum_load(uint32_t column, const float* place, bool live, uint32_t (&b)[16]) {
+  if constexpr (TWO) {
+    ts_ld16(column, b);                               // (the caller waits)
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float4 v = live ? __ldcg(reinterpret_cast<const float4*>(place) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      b[4 * i] = __float_as_uint(v.x); b[4 * i + 1] = __float_as_uint(v.y); b[4 * i + 2] = __float_as_uint(v.z); b[4 * i + 3] = __float_as_uint(v.w);
+    }
+  }
+}
+// The tensor core cuts off what a sum does not hold, up to 2^-23 of it at every 16 keys and always towards zero.  So O begins anew from time to
+// time, and what it held is added to a sum in 32 bits; the row's sum of weights with it.  kept: the reference of that sum, the sum of weights.
+// (Not inlined: the loop that calls it has no registers to spare.)
 template <class T, int D>
+__device__ __noinline__ void km_fold(uint32_t o, uint32_t column, float* place, bool live, bool first, float2* kept, float m, float l) {
+  constexpr bool TWO = KmShape<T, D>::kTwo;
+  const float f = first ? 0.f : km_exp2(kept->x - (m == -INFINITY ? 0.f : m));
+#pragma unroll 1
+  for (int c = 0; c < D / 16; c++) {
+    uint32_t a[16], b[16] = {};
+    if (!first) km_sum_load<TWO>(column + 16 * c, place + 16 * c, live, b);
+    __syncwarp();
+    ts_ld16(o + 16 * c, a);
+    ts_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; i++) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), f, __uint_as_float(a[i])));
+    if constexpr (TWO) {
+      ts_st16(column + 16 * c, a);
+    } else if (live) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        __stcg(reinterpret_cast<float4*>(place + 16 * c) + i, make_float4(__uint_as_float(a[4 * i]), __uint_as_float(a[4 * i + 1]),
+                                                                          __uint_as_float(a[4 * i + 2]), __uint_as_float(a[4 * i + 3])));
+    }
+    __syncwarp();
+  }
+  if constexpr (TWO) ts_wait_st();
+  *kept = make_float2(m, first ? l : fmaf(kept->y, f, l));
+}
+
+// FOLD: parts may have more than kFold tiles (a prompt of 4096 tokens, bf16: 403 us without the call in its loop, 411 with it)
+template <class T, int D, bool FOLD>
 __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_kernel(const Kv8AttnParams p) {
   using S = KmShape<T, D>;
   constexpr bool TWO = S::kTwo;
   extern __shared__ __align__(1024) uint8_t km_smem_raw[];
   uint8_t* smem = km_smem_raw + ((1024u - (smem_u32(km_smem_raw) & 1023u)) & 1023u);
   KmHead* hd = reinterpret_cast<KmHead*>(smem);
-  uint8_t* qs_mem = smem + 3072;                                       // [tiles][terms][kQ]
+  uint8_t* qs_mem = smem + kKmHeadBytes;                                      // [tiles][terms][kQ]
   uint8_t* kmem = qs_mem + S::kTiles * S::kTerms * S::kQ;              // [stages][kKv]
   uint8_t* vmem = kmem + kKmStages * S::kKv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -174,8 +222,8 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           for (int e = 0; e < S::kTerms; e++)
 #pragma unroll
             for (int k = 0; k < kKmKeys / 16; k++)
-              ts_mma_f16(tmem + (e ? S::kO2 : t * 256 + S::kO), tmem + (e ? S::kLow + b * 32 : t * 256 + b * kKmKeys) + k * 8,
-                         v_d + (uint32_t)(s * (S::kKv >> 4) + k * (2048 >> 4)), io, (j | k) ? 1u : 0u);
+              ts_mma_f16(tmem + (e ? S::kO2 : t * 256 + S::kO), tmem + t * 256 + b * kKmKeys + e * (kKmKeys / 2) + k * 8,
+                         v_d + (uint32_t)(s * (S::kKv >> 4) + k * (2048 >> 4)), io, ((e || !FOLD ? j : j % S::kFold) | k) ? 1u : 0u);
           ts_commit(j + 1 < n ? &hd->odone[t] : &hd->ofull[t]);
         }
         __syncwarp();
@@ -354,150 +402,162 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     const int first = p.window ? max(0, pos - p.window + 1) : 0, last = min(k1 - 1, pos);      // keys that the row sees
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-#pragma unroll 1
-    for (int j = 0; j < n; j++) {
-      const int s = j % kKmStages, base = k0 + kKmKeys * j;
-      const uint32_t ts = tmem + lanes + t * 256 + (j & 1) * kKmKeys;
-      ok = wait(&hd->sfull[t][j & 1], j >> 1, kDevWaitFull) && wait(&hd->vfull[s], j / kKmStages, kDevWaitFull);     // the scales come with the values
-      if (!ok) break;
-      __syncwarp();
-      ts_fence_after();
-      const bool cut = base + kKmKeys > all_hi || base < all_lo;
-      float mm = m == -INFINITY ? 0.f : m;
-      if (__any_sync(0xffffffffu, m == -INFINITY)) {   // no reference yet: the tile's largest exponent
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < kKmKeys / 16; c++) {
-          uint32_t a[16];
-          ts_ld16(ts + 16 * c, a);
-          ts_wait_ld();
-          const float4 sc = hd->sc[s][c];
-          const float f = f0 * sc.x;
-          const int hi = cut ? last - base - 16 * c : 16, lo = cut ? first - base - 16 * c : 0;
-#pragma unroll
-          for (int i = 0; i < 16; i++)
-            if (i <= hi && i >= lo) top = fmaxf(top, fmaf(__uint_as_float(a[i]), f, sc.y));
-          __syncwarp();
-        }
-        if (m == -INFINITY) m = floorf(top) - kKmFirst;
-        mm = m == -INFINITY ? 0.f : m;
+    for (int j0 = 0, j1; ok && j0 < n; j0 = j1) {
+      j1 = FOLD ? min(n, j0 + S::kFold) : n;
+      if (FOLD && j0) {
+        ok = wait(&hd->odone[t], j0 - 1, kDevWaitFull);
+        if (!ok) break;
+        __syncwarp();
+        ts_fence_after();
+        km_fold<T, D>(to, tmem + lanes + S::kSum, p.part + (((size_t)split * p.b.n_tokens + sq.row + tok) * p.heads + head) * D, live, j0 == S::kFold,
+                      &hd->kept[t * 128 + tr], m, l);
+        l = 0.f;
       }
-      // ---- weights.  The reference begins 7 below the first tile's largest exponent and stays unless the weights of 16 keys sum to more than
-      // 60000 (a half holds each of them below that).  Then those of the warp's rows that sum to more than 2^8 move up by a whole number, to a
-      // sum of 2^6 to 2^7, what has been summed against the old reference is scaled, and the weights are made again.  (Were only the row
-      // above 60000 moved, a prompt of 4096 tokens would take about 420 us instead of 403.)
-      // A half holds nothing below 2^-25, so N keys lose N 2^-31 at most beside the largest; the second halves of F32 weights, taken times
-      // 2^11, hold what is 2^11 below
-      bool lost = false;
-      int tries = 0;
-      uint32_t w[4][16];
-      float part[4];
 #pragma unroll 1
-      for (;;) {
-#pragma unroll
-        for (int h = 0; h < 4; h++) ts_ld16(ts + 16 * h, w[h]);
-        ts_wait_ld();
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-          const float4 sc = hd->sc[s][h];
-          const uint64_t f = kv8_two(f0 * sc.x, f0 * sc.x), b = kv8_two(sc.y - mm, sc.y - mm);
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float x, y;
-            kv8_apart(kv8_fma2(kv8_two(__uint_as_float(w[h][i]), __uint_as_float(w[h][i + 1])), f, b), x, y);
-            w[h][i] = __float_as_uint(x); w[h][i + 1] = __float_as_uint(y);
-          }
-        }
-        if (cut) {
-          const int hi = last - base, lo = first - base;
-#pragma unroll
-          for (int i = 0; i < 64; i++)
-            if (i > hi || i < lo) w[i >> 4][i & 15] = 0xFF800000u;
-          __syncwarp();
-        }
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-          uint64_t x[2] = {0, 0};
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float u = __uint_as_float(w[h][i]), v = __uint_as_float(w[h][i + 1]);
-            if (!TWO && (i & 6) == 6) km_exp2_fma(u, v);       // a quarter of them beside the others (F32 keeps its two units' accuracy)
-            else { u = km_exp2(u); v = km_exp2(v); }
-            w[h][i] = __float_as_uint(u); w[h][i + 1] = __float_as_uint(v);
-            x[i >> 1 & 1] = kv8_add2(x[i >> 1 & 1], kv8_two(u, v));
-          }
-          float y, z;
-          kv8_apart(kv8_add2(x[0], x[1]), y, z);
-          part[h] = y + z;
-        }
-        const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        if (!__any_sync(0xffffffffu, most > 60000.f && !lost)) break;
-        // by the next power of two above the sum, or, where that is beyond 32 bits or near the end of km_exp2_fma's range (which a sum then
-        // does not show to be passed), to the largest exponent.  A row whose products are infinite has none, and beyond 2^35 exponents are
-        // too coarse for one: after four times its weights stay what they are
-        constexpr float kFar = 100.f;
-        float up = most > 256.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) - kKmFirst : 0.f;
-        if (__any_sync(0xffffffffu, up > kFar)) {
+      for (int j = j0; j < j1; j++) {
+        const int s = j % kKmStages, base = k0 + kKmKeys * j;
+        const uint32_t ts = tmem + lanes + t * 256 + (j & 1) * kKmKeys;
+        ok = wait(&hd->sfull[t][j & 1], j >> 1, kDevWaitFull) && wait(&hd->vfull[s], j / kKmStages, kDevWaitFull);     // the scales come with the values
+        if (!ok) break;
+        __syncwarp();
+        ts_fence_after();
+        const bool cut = base + kKmKeys > all_hi || base < all_lo;
+        float mm = m == -INFINITY ? 0.f : m;
+        if (__any_sync(0xffffffffu, m == -INFINITY)) {   // no reference yet: the tile's largest exponent
           float top = -INFINITY;
 #pragma unroll 1
-          for (int k = 0; k < 4; k++) {
-            ts_ld16(ts + 16 * k, w[0]);
+          for (int c = 0; c < kKmKeys / 16; c++) {
+            uint32_t a[16];
+            ts_ld16(ts + 16 * c, a);
             ts_wait_ld();
-            const float4 sc = hd->sc[s][k];
+            const float4 sc = hd->sc[s][c];
+            const float f = f0 * sc.x;
+            const int hi = cut ? last - base - 16 * c : 16, lo = cut ? first - base - 16 * c : 0;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int key = base + 16 * k + i;
-              if (!cut || (key >= first && key <= last)) top = fmaxf(top, fmaf(__uint_as_float(w[0][i]), f0 * sc.x, sc.y - mm));
-            }
+            for (int i = 0; i < 16; i++)
+              if (i <= hi && i >= lo) top = fmaxf(top, fmaf(__uint_as_float(a[i]), f, sc.y));
             __syncwarp();
           }
-          if (up > kFar) {
-            lost = !(top < INFINITY);
-            up = lost ? 0.f : ceilf(top) - kKmFirst;
-          }
+          if (m == -INFINITY) m = floorf(top) - kKmFirst;
+          mm = m == -INFINITY ? 0.f : m;
         }
-        if (++tries == 4) lost = true;
-        const float f = km_exp2(-up);
-        m += up; mm = m; l *= f;
-        if (j) {                                       // the products of the tile before are there (those of two before are: this tile's scores are)
-          ok = wait(&hd->odone[t], j - 1, kDevWaitFull);
-          if (!ok) break;
-          __syncwarp();
-          ts_fence_after();
+        // ---- weights.  The reference begins 7 below the first tile's largest exponent and stays unless the weights of 16 keys sum to more than
+        // 60000 (a half holds each of them below that).  Then those of the warp's rows that sum to more than 2^8 move up by a whole number, to a
+        // sum of 2^6 to 2^7, what has been summed against the old reference is scaled, and the weights are made again.  (Were only the row
+        // above 60000 moved, a prompt of 4096 tokens would take about 420 us instead of 403.)
+        // A half holds nothing below 2^-25, so N keys lose N 2^-31 at most beside the largest; the second halves of F32 weights, taken times
+        // 2^11, hold what is 2^11 below
+        bool lost = false;
+        int tries = 0;
+        uint32_t w[4][16];
+        float part[4];
 #pragma unroll 1
-          for (int k = 0; k < S::kTerms * (D / 16); k++) {
-            const uint32_t at = k < D / 16 ? to + 16 * k : tmem + lanes + S::kO2 + 16 * (k - D / 16);
-            ts_ld16(at, w[0]);
-            ts_wait_ld();
+        for (;;) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[0][i] = __float_as_uint(__uint_as_float(w[0][i]) * f);
-            ts_st16(at, w[0]);
+          for (int h = 0; h < 4; h++) ts_ld16(ts + 16 * h, w[h]);
+          ts_wait_ld();
+#pragma unroll
+          for (int h = 0; h < 4; h++) {
+            const float4 sc = hd->sc[s][h];
+            const uint64_t f = kv8_two(f0 * sc.x, f0 * sc.x), b = kv8_two(sc.y - mm, sc.y - mm);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float x, y;
+              kv8_apart(kv8_fma2(kv8_two(__uint_as_float(w[h][i]), __uint_as_float(w[h][i + 1])), f, b), x, y);
+              w[h][i] = __float_as_uint(x); w[h][i + 1] = __float_as_uint(y);
+            }
           }
-          ts_wait_st();
-        }
-      }
-      if (!ok) break;
+          if (cut) {
+            const int hi = last - base, lo = first - base;
 #pragma unroll
-      for (int h = 0; h < 4; h++) l = fmaf(part[h], hd->sc[s][h].z, l);
+            for (int i = 0; i < 64; i++)
+              if (i > hi || i < lo) w[i >> 4][i & 15] = 0xFF800000u;
+            __syncwarp();
+          }
 #pragma unroll
-      for (int h = 0; h < 4; h += 2) {                 // in place of the products, all of which have been read
-        uint32_t hi[16], lo[16];
+          for (int h = 0; h < 4; h++) {
+            uint64_t x[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float u = __uint_as_float(w[h + (i >> 3)][2 * i & 15]), v = __uint_as_float(w[h + (i >> 3)][(2 * i & 15) + 1]);
-          hi[i] = km_pack(u, v);
-          if (TWO) {
-            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-            lo[i] = km_pack((u - y.x) * kKmLow, (v - y.y) * kKmLow);
+            for (int i = 0; i < 16; i += 2) {
+              float u = __uint_as_float(w[h][i]), v = __uint_as_float(w[h][i + 1]);
+              if (!TWO && (i & 6) == 6) km_exp2_fma(u, v);       // a quarter of them beside the others (F32 keeps its two units' accuracy)
+              else { u = km_exp2(u); v = km_exp2(v); }
+              w[h][i] = __float_as_uint(u); w[h][i + 1] = __float_as_uint(v);
+              x[i >> 1 & 1] = kv8_add2(x[i >> 1 & 1], kv8_two(u, v));
+            }
+            float y, z;
+            kv8_apart(kv8_add2(x[0], x[1]), y, z);
+            part[h] = y + z;
+          }
+          const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+          if (!__any_sync(0xffffffffu, most > 60000.f && !lost)) break;
+          // by the next power of two above the sum, or, where that is beyond 32 bits or near the end of km_exp2_fma's range (which a sum then
+          // does not show to be passed), to the largest exponent.  A row whose products are infinite has none, and beyond 2^35 exponents are
+          // too coarse for one: after four times its weights stay what they are
+          constexpr float kFar = 100.f;
+          float up = most > 256.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) - kKmFirst : 0.f;
+          if (__any_sync(0xffffffffu, up > kFar)) {
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+              ts_ld16(ts + 16 * k, w[0]);
+              ts_wait_ld();
+              const float4 sc = hd->sc[s][k];
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                const int key = base + 16 * k + i;
+                if (!cut || (key >= first && key <= last)) top = fmaxf(top, fmaf(__uint_as_float(w[0][i]), f0 * sc.x, sc.y - mm));
+              }
+              __syncwarp();
+            }
+            if (up > kFar) {
+              lost = !(top < INFINITY);
+              up = lost ? 0.f : ceilf(top) - kKmFirst;
+            }
+          }
+          if (++tries == 4) lost = true;
+          const float f = km_exp2(-up);
+          m += up; mm = m; l *= f;
+          if (j) {                                       // the products of the tile before are there (those of two before are: this tile's scores are)
+            ok = wait(&hd->odone[t], j - 1, kDevWaitFull);
+            if (!ok) break;
+            __syncwarp();
+            ts_fence_after();
+#pragma unroll 1
+            for (int k = 0; k < S::kTerms * (D / 16); k++) {
+              const uint32_t at = k < D / 16 ? to + 16 * k : tmem + lanes + S::kO2 + 16 * (k - D / 16);
+              ts_ld16(at, w[0]);
+              ts_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; i++) w[0][i] = __float_as_uint(__uint_as_float(w[0][i]) * f);
+              ts_st16(at, w[0]);
+            }
+            ts_wait_st();
           }
         }
-        ts_st16(ts + 8 * h, hi);
-        if constexpr (TWO) ts_st16(tmem + lanes + S::kLow + (j & 1) * 32 + 8 * h, lo);
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < 4; h++) l = fmaf(part[h], hd->sc[s][h].z, l);
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {                 // in place of the products, all of which have been read
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float u = __uint_as_float(w[h + (i >> 3)][2 * i & 15]), v = __uint_as_float(w[h + (i >> 3)][(2 * i & 15) + 1]);
+            hi[i] = km_pack(u, v);
+            if (TWO) {
+              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+              lo[i] = km_pack((u - y.x) * kKmLow, (v - y.y) * kKmLow);
+            }
+          }
+          ts_st16(ts + 8 * h, hi);
+          if constexpr (TWO) ts_st16(ts + kKmKeys / 2 + 8 * h, lo);
+        }
+        ts_wait_st();
+        ts_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&hd->pfull[t][j & 1]);
       }
-      ts_wait_st();
-      ts_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&hd->pfull[t][j & 1]);
     }
     ok = ok && wait(&hd->ofull[t], 0, kDevWaitFull);
     if (ok) {
@@ -505,7 +565,12 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
       ts_fence_after();
       const bool whole = p.splits == 1;
       const size_t at = ((size_t)split * p.b.n_tokens + sq.row + tok) * p.heads + head;
-      float mul = 1.f;
+      float mul = 1.f, f_sum = 0.f;
+      if (FOLD && n > S::kFold) {
+        const float2 kept = hd->kept[t * 128 + tr];
+        f_sum = km_exp2(kept.x - (m == -INFINITY ? 0.f : m));
+        l = fmaf(kept.y, f_sum, l);
+      }
       if (whole) {
         float sum = l;
         if (p.sinks) sum += km_exp2(p.sinks[head] * kLog2e - (m == -INFINITY ? 0.f : m));
@@ -529,6 +594,13 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           ts_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; i++) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), 1.f / kKmLow, __uint_as_float(a[i])));
+        }
+        if (FOLD && n > S::kFold) {
+          uint32_t b[16];
+          km_sum_load<TWO>(tmem + lanes + S::kSum + 16 * c, p.part + at * D + 16 * c, live, b);
+          ts_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i++) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), f_sum, __uint_as_float(a[i])));
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -576,10 +648,10 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
   }
 }
 
-template <class T, int D>
+template <class T, int D, bool FOLD>
 static int launch_many(const Kv8AttnParams& p, int groups, cudaStream_t st, int dev) {
   using S = KmShape<T, D>;
-  auto kern = kv8_attn_many_kernel<T, D>;
+  auto kern = kv8_attn_many_kernel<T, D, FOLD>;
   const int smem = std::max(S::kSmem, 120 * 1024);       // one block an SM: it takes the whole tensor memory
   static bool done[64] = {};
   if (!done[dev & 63]) {
@@ -592,9 +664,13 @@ static int launch_many(const Kv8AttnParams& p, int groups, cudaStream_t st, int 
 }
 static_assert(kKv8ManyRowsF32 == kKmRows && kKv8ManyRows == 2 * kKmRows, "row tiles of a block");
 int kv8_attn_many(const Kv8AttnParams& p, int groups, int elem_type, int D, cudaStream_t st, int dev) {
-  if (elem_type == F32) return D == 64 ? launch_many<float, 64>(p, groups, st, dev) : launch_many<float, 128>(p, groups, st, dev);
-  if (elem_type == F16) return D == 64 ? launch_many<__half, 64>(p, groups, st, dev) : launch_many<__half, 128>(p, groups, st, dev);
-  return D == 64 ? launch_many<__nv_bfloat16, 64>(p, groups, st, dev) : launch_many<__nv_bfloat16, 128>(p, groups, st, dev);
+  const bool fold = p.chunk > kKv8Fold;
+#define KM_GO(T, FOLD) return D == 64 ? launch_many<T, 64, FOLD>(p, groups, st, dev) : launch_many<T, 128, FOLD>(p, groups, st, dev)
+  if (elem_type == F32) KM_GO(float, true);
+  if (elem_type == F16) { if (fold) KM_GO(__half, true); KM_GO(__half, false); }
+  if (fold) KM_GO(__nv_bfloat16, true);
+  KM_GO(__nv_bfloat16, false);
+#undef KM_GO
 }
 
 }  // namespace msb

@@ -99,3 +99,55 @@ def test_attention_keeps_small_weights_beside_a_large_one(S, n, dt, gap):
         tol = (weight + (L / 8 + 32) * 2.0 ** -23) * ref + share * gap * 2.0 ** -21
         got = out.view(S, n, 64, 128)[:, :, h].double()
         assert ((got - ref).abs() <= tol * (1 + half) + half * ref.abs() + tiny).all(), (h, float((got - ref).abs().max()), float(tol.max()))
+
+
+@pytest.mark.parametrize("S,n", ((128, 1), (1, 512)))
+def test_attention_sums_of_f32_rows_keep_what_is_below_their_last_bit(S, n):
+    """Tens of thousands of weights, each of them below the last bit of the first key's, that together are not.
+
+    As above; but sums are begun anew after 1024 keys at most (few rows: 512 of a warp's), and what each held is added in 32 bits."""
+    from macseek_b200 import kv8
+    L, gap = 40000, 20.0
+    cache, batch, q, v = one_long_context(S, n, L, "f32")
+    out, e = torch.zeros_like(q), enc()
+    kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 64), scale=gap)
+    e.wait()
+    pos = torch.arange(L - n, L, device="cuda")
+    small = float(torch.exp(torch.tensor(-gap, dtype=torch.float64)))
+    total = 1 + small * pos.double()[:, None]
+    adds = L / 1024 if n > 1 else L / 4 / 512                        # (a warp of a block of few rows has a quarter of a part's keys)
+    for h in range(0, 64, 7):
+        ref = (v[h // 8, 0] + small * v[h // 8, 1:].cumsum(0)[pos - 1]) / total
+        tol = (2.0 ** -21 + 2.0 ** -20 + (1024 / 8 + 32) * 2.0 ** -23 + adds * 2.0 ** -24) * ref + (total - 1) / total * gap * 2.0 ** -21
+        assert ((out.view(S, n, 64, 128)[:, :, h].double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("S,n,kv,dim,L", ((128, 1, 8, 128, 200000), (1, 512, 8, 128, 200000), (1, 256, 1, 64, 400000)))
+def test_attention_of_long_contexts_is_not_biased(S, n, kv, dim, L, dt):
+    """Values of one sign under random weights: what sums cut off would make every output smaller.  (One part, several, and parts of many rows whose
+    sums are begun anew.)
+
+    Roundings of weights and outputs cancel in the mean (two heads, 64 rows, their dims: their mean is below 2^-11 / 60); what does not is 2^-23 of
+    a sum at every 16 keys, for 1024 keys of F32 rows and 16384 of others, and 2^-18 of a weight."""
+    from macseek_b200 import kv8
+    sc, G = dim ** -0.5, 8
+    cache, batch, q, v = one_long_context(S, n, L, dt, kv=kv, dim=dim)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    cache.k.copy_(torch.randn(cache.k.shape, generator=g, device="cuda").to(R.FP8).view(torch.uint8))
+    q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+    out, e = torch.zeros_like(q), enc()
+    scratch = kv8.attn_scratch(cache, batch, kv * G)
+    scratch.fill_(255)                                               # NaN
+    kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, scale=sc)
+    e.wait()
+    err = []
+    for h in (3, kv * G - 4):
+        k = R.values(cache.k)[:, h // G].reshape(-1, dim)[:L]
+        rows = torch.arange(S * n - 64, S * n, device="cuda")
+        lg = (q[rows, h].double() @ k.T * sc).masked_fill(torch.arange(L, device="cuda")[None] > (L - n + rows % n)[:, None], -torch.inf)
+        ref = torch.softmax(lg, 1) @ v[h // G]
+        err.append((out[rows, h].double() / ref - 1).mean())
+    keys = 1024 if dt == "f32" else 16384
+    bias = abs(float(torch.stack(err).mean()))
+    assert bias <= keys / 16 * 2.0 ** -23 + 2.0 ** -18 + (0 if dt == "f32" else R.half_step(R.DT[dt])[0] / 60), bias
