@@ -310,8 +310,9 @@ typedef struct {
  * are the last ones of its kv_len[s] tokens; token p lies in block table[s][p / block].  The arrays are device memory (they
  * may change between replays of a captured call); max_new and max_len bound the rows and tokens of any sequence.  Rows
  * behind seq_start[n_seq] are padding: never read, never written.  A sequence whose numbers cannot be right (a start that
- * falls or lies outside [0, n_tokens], more rows than max_new or than tokens, more tokens than max_len) is left out, and a
- * block id outside [0, n_blocks) is a block that is not there; both set device status 4. */
+ * falls or lies outside [0, n_tokens], more rows than max_new or than tokens, more tokens than max_len) is left out (rows
+ * that two right ones share, which takes a start that falls, are undefined), and a block id outside [0, n_blocks) is a block
+ * that is not there; both set device status 4. */
 typedef struct {
   int n_seq, n_tokens, max_new, max_len;
   const int* seq_start;                  /* int32[n_seq + 1] */

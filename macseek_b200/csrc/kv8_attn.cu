@@ -446,10 +446,11 @@ __global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnParams 
   const int tok = (int)(at / p.heads), head = (int)(at - (int64_t)tok * p.heads);
   int n = 0;
   if (tok < p.b.n_tokens) {
-    const int s = kv8_find(p.b.n_seq, tok, [&](int i) { return __ldg(p.b.seq_start + i); });
-    const Kv8Seq sq = kv8_seq(p.b, s, p.status);
+    Kv8Seq sq;
+    const int s = kv8_owner(p.b.n_seq, tok, [&](int i) { return kv8_seq(p.b, i, p.status); }, [&](int i) { return __ldg(p.b.seq_start + i); },
+                            [](auto f) { return __ballot_sync(0xffffffffu, f(threadIdx.x & 31)); }, sq);
     const int i = tok - sq.row;
-    if (i >= 0 && i < sq.n) {
+    if (s >= 0) {
       const int row = i * p.G + head % p.G, m0 = row / p.tile * p.tile, m1 = min(m0 + p.tile, sq.n * p.G);
       const Kv8Range kr = kv8_range(sq, m0, m1, p.G, p.window, p.step);
       n = (kr.hi - kr.lo + p.chunk - 1) / p.chunk;

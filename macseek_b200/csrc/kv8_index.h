@@ -57,6 +57,26 @@ KV8_HD int kv8_search(int n, int x, First first, Ballot ballot) {
   return lo;
 }
 
+// The sequence that owns row x (-1: none): found by its start, and where starts that fall mislead the search, the first right one that has it.
+template <class SeqOf, class Start, class Ballot>
+KV8_HD int kv8_owner(int n, int x, SeqOf seq, Start start, Ballot ballot, Kv8Seq& q) {
+  int s = kv8_search(n, x, start, ballot);
+  q = seq(s);
+  if (x >= q.row && x - q.row < q.n) return s;
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    unsigned m = ballot([&](int lane) {
+      if (s0 + lane >= n) return false;
+      const Kv8Seq o = seq(s0 + lane);
+      return x >= o.row && x - o.row < o.n;
+    });
+    if (m == 0) continue;
+    for (s = s0; !(m & 1); m >>= 1) s++;
+    q = seq(s);
+    return s;
+  }
+  return -1;
+}
+
 // Keys that rows [m0, m1) of a sequence look at (row r is token r / G of its new ones): [lo, hi), lo rounded down to `step`.
 struct Kv8Range { int lo, hi; };
 KV8_HD Kv8Range kv8_range(const Kv8Seq& s, int m0, int m1, int G, int window, int step) {

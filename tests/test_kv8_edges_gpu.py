@@ -151,3 +151,40 @@ def test_attention_of_long_contexts_is_not_biased(S, n, kv, dim, L, dt):
     keys = 1024 if dt == "f32" else 16384
     bias = abs(float(torch.stack(err).mean()))
     assert bias <= keys / 16 * 2.0 ** -23 + 2.0 ** -18 + (0 if dt == "f32" else R.half_step(R.DT[dt])[0] / 60), bias
+
+
+def broken_starts(c):
+    """(start's entries to change, the sequences that are right then)."""
+    n = len(c.seqs)
+    yield {2: c.rows + 70}, [s for s in range(n) if s not in (1, 2)]
+    yield {2: 10 ** 6}, [s for s in range(n) if s not in (1, 2)]
+    yield {1: -3, n - 1: 2 ** 31 - 1}, [s for s in range(n) if s not in (0, 1, n - 2, n - 1)]
+    yield {3: 0}, [s for s in range(n) if s not in (2, 3)]             # (sequence 3 would have more rows than any may)
+
+
+@pytest.mark.parametrize("seqs,G", (([(5, 2000 + 7 * i) for i in range(7)], 8), ([(1, 900), (3, 700), (2, 1000), (1, 50), (4, 800)], 2), ([(80, 3000)] * 5, 8)))
+def test_broken_starts_leave_the_other_sequences_right_in_several_parts(seqs, G):
+    """A start that falls or lies outside hides no sequence behind it from the kernel that joins parts."""
+    from macseek_b200 import _lib, kv8
+    c = R.Case(seqs, 2, 64, 16, seed=11, pad=3)
+    e, q = enc(), c.randn(c.rows, 2 * G, 64)
+    outs = []
+    start = c.start.clone()
+    for change, good in [({}, range(len(seqs)))] + list(broken_starts(c)):
+        c.start.copy_(start)
+        for i, x in change.items():
+            c.start[i] = x
+        cache, batch = c.cache(), c.batch()
+        out = torch.full_like(q, 7)
+        scratch = kv8.attn_scratch(cache, batch, 2 * G)
+        scratch.fill_(255)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, scratch)
+        torch.cuda.synchronize()
+        assert _lib.device_status() == (4 if change else 0)
+        if not change:
+            check_attn(c, q, out, torch.full_like(q, 7), 0.125, 0, None)
+        outs.append(out)
+        for s in good:
+            r = slice(c.start_host[s], c.start_host[s] + seqs[s][0])
+            assert torch.equal(out[r], outs[0][r]), (change, s)
+        assert (out[c.start_host[-1]:] == 7).all()

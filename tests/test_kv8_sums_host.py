@@ -41,3 +41,66 @@ int main() {
   puts("ok");
 }
 """)
+
+
+BATCH = r"""
+#include "kv8_index.h"
+#include <algorithm>
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+using namespace msb;
+static void need(bool ok, const char* what, int line) { if (!ok) { printf("%s (line %d)\n", what, line); exit(1); } }
+#define NEED(x) need(x, #x, __LINE__)
+struct Host { template <class F> unsigned operator()(F f) const { unsigned m = 0; for (int l = 0; l < 32; l++) if (f(l)) m |= 1u << l; return m; } };
+struct Batch {
+  std::vector<int> start{0}, len;
+  int n_seq, n_tokens, max_new = 1, max_len = 1;
+  template <class R> Batch(R& upto, bool broken) {
+    n_seq = upto(9) == 0 ? 1 + upto(1500) : 1 + upto(70);
+    const int most = upto(3) ? 1 + upto(5) : 1 + upto(400), ctx = upto(1) ? upto(700) : 0;
+    for (int s = 0; s < n_seq; s++) {
+      const int n = upto(most), l = n + upto(ctx);
+      start.push_back(start.back() + n); len.push_back(l);
+      max_new = kv8_max(max_new, n); max_len = kv8_max(max_len, l);
+    }
+    n_tokens = kv8_max(start.back() + upto(3), max_new);
+    if (broken)
+      for (int k = 0; k < 1 + upto(3); k++) {
+        const int junk[7] = {-1, -2147483647 - 1, 2147483647, n_tokens + 1, 7, max_len + 1, upto(n_tokens)};
+        if (upto(3)) start[upto(n_seq)] = junk[upto(6)];
+        else len[upto(n_seq - 1)] = junk[upto(6)];
+      }
+  }
+  Kv8Seq seq(int s) const {
+    Kv8Seq q;
+    kv8_seq_of(start[s], start[s + 1], len[s], n_tokens, max_new, max_len, q);
+    return q;
+  }
+};
+"""
+
+
+def test_every_row_of_a_right_sequence_has_an_owner_in_broken_batches(tmp_path):
+    run(tmp_path, BATCH + r"""
+int main() {
+  std::mt19937 rng(7);
+  auto upto = [&](int n) { return (int)(rng() % (unsigned)(n + 1)); };
+  for (int trial = 0; trial < 3000; trial++) {
+    const Batch b(upto, trial % 4 != 0);
+    std::vector<int> owners(b.n_tokens, 0);
+    for (int s = 0; s < b.n_seq; s++) { const Kv8Seq q = b.seq(s); for (int i = 0; i < q.n; i++) owners[q.row + i]++; }
+    for (int k = 0; k < 200; k++) {
+      const int x = upto(b.n_tokens - 1);
+      Kv8Seq q;
+      const int s = kv8_owner(b.n_seq, x, [&](int i) { NEED(i >= 0 && i < b.n_seq); return b.seq(i); }, [&](int i) { return b.start[i]; }, Host(), q);
+      NEED((s >= 0) == (owners[x] > 0));
+      if (s < 0) continue;
+      const Kv8Seq o = b.seq(s);
+      NEED(o.row == q.row && o.n == q.n && o.len == q.len && x >= o.row && x < o.row + o.n);
+    }
+  }
+  puts("ok");
+}
+""")
