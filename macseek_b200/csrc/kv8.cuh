@@ -41,20 +41,39 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Batch& b, int s, int* status)
     atomicCAS(status, 0, kDevBadBatch);
   return q;
 }
-template <class F>
-__device__ __forceinline__ int kv8_find(int n, int x, F first) {       // by whole warps
-  return kv8_search(n, x, first, [](auto f) { return __ballot_sync(0xffffffffu, f(threadIdx.x & 31)); });
-}
-// Work item `item` (kv8_index.h): `each` > 0: sequence item / each, its item % each; 0: found among the sequences' first items.  By whole warps.
-__device__ __forceinline__ Kv8Item kv8_item(const Kv8Batch& b, int shift, int each, int item, int* status, int& s) {
-  if (each) {
-    s = item / each;
-    return kv8_item_of(kv8_seq(b, s, status), item - s * each, shift);
+// The items of a block of threads, by whole warps.  `each` > 0: item `item` is sequence item / each's.  0: item - 1 is found among the sequences'
+// first items, and the block of item 0 looks the batch through: what the others miss, which takes starts that fall, it does itself.
+struct Kv8Items {
+  int s = 0, j = 0;               // item 0: where the batch has been looked through to; j -1: the only item is done
+  __device__ __forceinline__ bool next(const Kv8Batch& b, int shift, int each, int item, int* status, int& seq, Kv8Item& it) {
+    const auto ballot = [](auto f) { return __ballot_sync(0xffffffffu, f(threadIdx.x & 31)); };
+    const auto start = [&](int i) { return __ldg(b.seq_start + i); };
+    if (each || item) {
+      if (j < 0) return false;
+      j = -1;
+      if (each) {
+        seq = item / each;
+        it = kv8_item_of(kv8_seq(b, seq, status), item - seq * each, shift);
+      } else {
+        const auto first = [&](int i) { return kv8_first_item(start(i), i, shift); };
+        seq = kv8_search(b.n_seq, item - 1, first, ballot);
+        it = kv8_item_of(kv8_seq(b, seq, status), item - 1 - first(seq), shift);
+      }
+      return it.n != 0;
+    }
+    if (s == 0 && j == 0) {
+      bool falls = false;
+      for (int i = threadIdx.x & 31; i < b.n_seq; i += 32) {
+        falls |= start(i + 1) < start(i);
+        kv8_seq(b, i, status);                                          // (recorded, whether or not an item is found to be its)
+      }
+      if (!__any_sync(0xffffffffu, falls)) return false;
+    }
+    const bool more = kv8_next_missed(b.n_seq, shift, [&](int i) { return kv8_seq(b, i, status); }, start, ballot, s, j, it);
+    seq = s;
+    return more;
   }
-  auto first = [&](int i) { return kv8_first_item(__ldg(b.seq_start + i), i, shift); };
-  s = kv8_find(b.n_seq, item, first);
-  return kv8_item_of(kv8_seq(b, s, status), item - first(s), shift);
-}
+};
 // The block of an item of sequence s (-1: not there).
 __device__ __forceinline__ int kv8_block(const Kv8Batch& b, int n_blocks, int s, const Kv8Item& it, int* status) {
   const int id = __ldg(b.table + (size_t)s * b.table_stride + it.blk);

@@ -48,7 +48,7 @@ struct Kv8RowsParams {
   void *k, *v;                    // rows (read by the writing kernel, written by the reading one)
   int64_t k_stride, v_stride;     // elements
   int k_vec, v_vec;
-  int each;                       // items of a sequence, 0: as kv8_item finds them
+  int each;                       // items of a sequence, 0: as Kv8Items finds them
   int* status;
 };
 
@@ -64,107 +64,108 @@ __global__ void __launch_bounds__(kv8_block_threads(THREADS)) kv8_write_kernel(c
   __shared__ float s_top[kGroups][2][kWarps];
   float (&s_max)[2][kWarps] = s_top[threadIdx.x / THREADS];
   const int tid = threadIdx.x % THREADS, sh = p.c.shift, units = 2 * p.c.heads, step = gridDim.y * kGroups;
-  int s;
-  const Kv8Item it = kv8_item(p.b, sh, p.each, blockIdx.x, p.status, s);
-  if (it.n == 0) return;
-  const int pieces = it.n * kRow;
-  typename Elems<T>::Raw r[MOST], next[MOST];
-  auto load = [&](int u) {        // unit u: head u / 2, its keys or its values
-    const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
-    const int64_t stride = values ? p.v_stride : p.k_stride;
-    const T* rows = static_cast<const T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
-    if (vec) {
+  Kv8Items items;
+  Kv8Item it;
+  for (int s, turn = 0; items.next(p.b, sh, p.each, blockIdx.x, p.status, s, it);) {
+    const int pieces = it.n * kRow;
+    typename Elems<T>::Raw r[MOST], next[MOST];
+    auto load = [&](int u) {        // unit u: head u / 2, its keys or its values
+      const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
+      const int64_t stride = values ? p.v_stride : p.k_stride;
+      const T* rows = static_cast<const T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
+      if (vec) {
+#pragma unroll
+        for (int i = 0; i < MOST; i++) {
+          const int c = tid + i * THREADS;
+          if (c < pieces) next[i] = Elems<T>::raw(rows + (c / kRow) * stride + c % kRow * 8);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MOST; i++) {
+          const int c = tid + i * THREADS;
+          if (c < pieces) next[i] = Elems<T>::gather(rows + (c / kRow) * stride + c % kRow * 8);
+        }
+      }
+    };
+    int u = blockIdx.y * kGroups + threadIdx.x / THREADS;
+    if (u < units) load(u);
+    const int id = kv8_block(p.b, p.c.n_blocks, s, it, p.status);
+    if (id < 0) continue;
+    float was = 0.f;
+    if (it.at && u < units) was = ((u & 1) ? p.c.vs : p.c.ks)[(size_t)id * p.c.heads + (u >> 1)];
+    for (; u < units; u += step, turn ^= 1) {
+      const size_t head = (size_t)id * p.c.heads + (u >> 1);
+      uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D;
+      float* scale = ((u & 1) ? p.c.vs : p.c.ks) + head;
+      const float old = was;
+#pragma unroll
+      for (int i = 0; i < MOST; i++) r[i] = next[i];
+      if (u + step < units) {
+        load(u + step);
+        if (it.at) was = (((u + step) & 1) ? p.c.vs : p.c.ks)[(size_t)id * p.c.heads + ((u + step) >> 1)];
+      }
+      float top = 0.f;
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < MOST; i++)
+        if (tid + i * THREADS < pieces) {
+          float v[8];
+          Elems<T>::open(r[i], v);
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const float a = fabsf(v[j]);
+            nan |= a != a;
+            if (a <= 3.402823466e38f) top = fmaxf(top, a);            // an infinity becomes the largest code
+          }
+        }
+      top = warp_max(top);
+      if (THREADS > 32) {
+        if ((tid & 31) == 0) s_max[turn][tid >> 5] = top;
+        bar_sync_named(1 + threadIdx.x / THREADS, THREADS);           // (also: every thread has read the scale that is written below)
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) top = fmaxf(top, s_max[turn][i]);
+      }
+      // top = 1.m * 2^e <= 448 * 2^E = 1.75 * 2^(8 + E)
+      const uint32_t bits = __float_as_uint(top);
+      int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+      e = min(max(e, kKv8MinExp), kKv8MaxExp);
+      int e_old = e;
+      if (it.at) { e_old = kv8_exp(old); e = max(e, e_old); }
+      const float inv = kv8_pow2(-e);
 #pragma unroll
       for (int i = 0; i < MOST; i++) {
         const int c = tid + i * THREADS;
-        if (c < pieces) next[i] = Elems<T>::raw(rows + (c / kRow) * stride + c % kRow * 8);
-      }
-    } else {
+        if (c < pieces) {
+          float v[8];
+          Elems<T>::open(r[i], v);
 #pragma unroll
-      for (int i = 0; i < MOST; i++) {
-        const int c = tid + i * THREADS;
-        if (c < pieces) next[i] = Elems<T>::gather(rows + (c / kRow) * stride + c % kRow * 8);
-      }
-    }
-  };
-  int u = blockIdx.y * kGroups + threadIdx.x / THREADS;
-  if (u < units) load(u);
-  const int id = kv8_block(p.b, p.c.n_blocks, s, it, p.status);
-  if (id < 0) return;
-  float was = 0.f;
-  if (it.at && u < units) was = ((u & 1) ? p.c.vs : p.c.ks)[(size_t)id * p.c.heads + (u >> 1)];
-  for (int turn = 0; u < units; u += step, turn ^= 1) {
-    const size_t head = (size_t)id * p.c.heads + (u >> 1);
-    uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D;
-    float* scale = ((u & 1) ? p.c.vs : p.c.ks) + head;
-    const float old = was;
+          for (int j = 0; j < 8; j++) v[j] *= inv;
+          if (nan) {                                                  // the cache holds none: its attention multiplies masked rows by 0
 #pragma unroll
-    for (int i = 0; i < MOST; i++) r[i] = next[i];
-    if (u + step < units) {
-      load(u + step);
-      if (it.at) was = (((u + step) & 1) ? p.c.vs : p.c.ks)[(size_t)id * p.c.heads + ((u + step) >> 1)];
-    }
-    float top = 0.f;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < MOST; i++)
-      if (tid + i * THREADS < pieces) {
-        float v[8];
-        Elems<T>::open(r[i], v);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float a = fabsf(v[j]);
-          nan |= a != a;
-          if (a <= 3.402823466e38f) top = fmaxf(top, a);            // an infinity becomes the largest code
+            for (int j = 0; j < 8; j++) v[j] = v[j] != v[j] ? 0.f : v[j];
+          }
+          *reinterpret_cast<uint2*>(codes + (it.at + c / kRow) * D + c % kRow * 8) =
+              make_uint2(kv8_codes4(v[0], v[1], v[2], v[3]), kv8_codes4(v[4], v[5], v[6], v[7]));
         }
       }
-    top = warp_max(top);
-    if (THREADS > 32) {
-      if ((tid & 31) == 0) s_max[turn][tid >> 5] = top;
-      bar_sync_named(1 + threadIdx.x / THREADS, THREADS);           // (also: every thread has read the scale that is written below)
-#pragma unroll
-      for (int i = 0; i < kWarps; i++) top = fmaxf(top, s_max[turn][i]);
-    }
-    // top = 1.m * 2^e <= 448 * 2^E = 1.75 * 2^(8 + E)
-    const uint32_t bits = __float_as_uint(top);
-    int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    e = min(max(e, kKv8MinExp), kKv8MaxExp);
-    int e_old = e;
-    if (it.at) { e_old = kv8_exp(old); e = max(e, e_old); }
-    const float inv = kv8_pow2(-e);
-#pragma unroll
-    for (int i = 0; i < MOST; i++) {
-      const int c = tid + i * THREADS;
-      if (c < pieces) {
-        float v[8];
-        Elems<T>::open(r[i], v);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= inv;
-        if (nan) {                                                  // the cache holds none: its attention multiplies masked rows by 0
-#pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = v[j] != v[j] ? 0.f : v[j];
-        }
-        *reinterpret_cast<uint2*>(codes + (it.at + c / kRow) * D + c % kRow * 8) =
-            make_uint2(kv8_codes4(v[0], v[1], v[2], v[3]), kv8_codes4(v[4], v[5], v[6], v[7]));
-      }
-    }
-    if (nan) atomicCAS(p.status, 0, kDevNan);
-    if (e > e_old) {                                                // older tokens of the block move to the larger scale
-      const float f = kv8_pow2(e_old - e);
+      if (nan) atomicCAS(p.status, 0, kDevNan);
+      if (e > e_old) {                                                // older tokens of the block move to the larger scale
+        const float f = kv8_pow2(e_old - e);
 #pragma unroll 4
-      for (int c = tid; c < it.at * (D / 16); c += THREADS) {
-        uint4* q = reinterpret_cast<uint4*>(codes) + c;
-        uint32_t w[4] = {q->x, q->y, q->z, q->w};
+        for (int c = tid; c < it.at * (D / 16); c += THREADS) {
+          uint4* q = reinterpret_cast<uint4*>(codes) + c;
+          uint32_t w[4] = {q->x, q->y, q->z, q->w};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 a = kv8_float2(w[j]), b = kv8_float2(w[j] >> 16);
-          w[j] = kv8_codes4(a.x * f, a.y * f, b.x * f, b.y * f);
+          for (int j = 0; j < 4; j++) {
+            const float2 a = kv8_float2(w[j]), b = kv8_float2(w[j] >> 16);
+            w[j] = kv8_codes4(a.x * f, a.y * f, b.x * f, b.y * f);
+          }
+          *q = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        *q = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      if (THREADS == 32) __syncwarp();
+      if (tid == 0) *scale = kv8_pow2(e);
     }
-    if (THREADS == 32) __syncwarp();
-    if (tid == 0) *scale = kv8_pow2(e);
   }
 }
 
@@ -175,53 +176,54 @@ __global__ void __launch_bounds__(kKv8Threads) kv8_read_kernel(const Kv8RowsPara
   pdl_wait();
   constexpr int V = 16 / sizeof(T), kRow = D / V, kGroups = kKv8Threads / THREADS;
   const int sh = p.c.shift, units = 2 * p.c.heads, tid = threadIdx.x % THREADS, step = gridDim.y * kGroups;
-  int s;
-  const Kv8Item it = kv8_item(p.b, sh, p.each, blockIdx.x, p.status, s);
-  if (it.n == 0) return;
-  const int id = kv8_block(p.b, p.c.n_blocks, s, it, p.status), pieces = it.n * kRow;
-  uint32_t w[MOST][V / 4], next[MOST][V / 4] = {};
-  float scale = 0.f, next_scale = 0.f;
-  auto load = [&](int u) {
-    if (id < 0) return;
-    const size_t head = (size_t)id * p.c.heads + (u >> 1);
-    const uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D + it.at * D;
+  Kv8Items items;
+  Kv8Item it;
+  for (int s; items.next(p.b, sh, p.each, blockIdx.x, p.status, s, it);) {
+    const int id = kv8_block(p.b, p.c.n_blocks, s, it, p.status), pieces = it.n * kRow;
+    uint32_t w[MOST][V / 4], next[MOST][V / 4] = {};
+    float scale = 0.f, next_scale = 0.f;
+    auto load = [&](int u) {
+      if (id < 0) return;
+      const size_t head = (size_t)id * p.c.heads + (u >> 1);
+      const uint8_t* codes = ((u & 1) ? p.c.v : p.c.k) + (head << sh) * D + it.at * D;
 #pragma unroll
-    for (int i = 0; i < MOST; i++) {
-      const int c = tid + i * THREADS;
-      if (c < pieces) {
-        if (V == 8) {
-          const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes) + c);
-          next[i][0] = q.x; next[i][V / 4 - 1] = q.y;
-        } else {
-          next[i][0] = __ldg(reinterpret_cast<const uint32_t*>(codes) + c);
+      for (int i = 0; i < MOST; i++) {
+        const int c = tid + i * THREADS;
+        if (c < pieces) {
+          if (V == 8) {
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes) + c);
+            next[i][0] = q.x; next[i][V / 4 - 1] = q.y;
+          } else {
+            next[i][0] = __ldg(reinterpret_cast<const uint32_t*>(codes) + c);
+          }
         }
       }
-    }
-    next_scale = __ldg(((u & 1) ? p.c.vs : p.c.ks) + head);
-  };
-  int u = blockIdx.y * kGroups + threadIdx.x / THREADS;
-  if (u < units) load(u);
-  for (; u < units; u += step) {
+      next_scale = __ldg(((u & 1) ? p.c.vs : p.c.ks) + head);
+    };
+    int u = blockIdx.y * kGroups + threadIdx.x / THREADS;
+    if (u < units) load(u);
+    for (; u < units; u += step) {
 #pragma unroll
-    for (int i = 0; i < MOST; i++)
+      for (int i = 0; i < MOST; i++)
 #pragma unroll
-      for (int j = 0; j < V / 4; j++) w[i][j] = next[i][j];
-    scale = next_scale;
-    if (u + step < units) load(u + step);
-    const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
-    const int64_t stride = values ? p.v_stride : p.k_stride;
-    T* rows = static_cast<T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
+        for (int j = 0; j < V / 4; j++) w[i][j] = next[i][j];
+      scale = next_scale;
+      if (u + step < units) load(u + step);
+      const bool values = u & 1, vec = values ? p.v_vec : p.k_vec;
+      const int64_t stride = values ? p.v_stride : p.k_stride;
+      T* rows = static_cast<T*>(values ? p.v : p.k) + it.row * stride + (u >> 1) * D;
 #pragma unroll
-    for (int i = 0; i < MOST; i++) {
-      const int c = tid + i * THREADS;
-      if (c >= pieces) break;
-      float o[V];
+      for (int i = 0; i < MOST; i++) {
+        const int c = tid + i * THREADS;
+        if (c >= pieces) break;
+        float o[V];
 #pragma unroll
-      for (int j = 0; j < V / 2; j++) {
-        const float2 a = kv8_float2(w[i][j >> 1] >> (16 * (j & 1)));
-        o[2 * j] = a.x * scale; o[2 * j + 1] = a.y * scale;
+        for (int j = 0; j < V / 2; j++) {
+          const float2 a = kv8_float2(w[i][j >> 1] >> (16 * (j & 1)));
+          o[2 * j] = a.x * scale; o[2 * j + 1] = a.y * scale;
+        }
+        Elems<T>::store16(rows + (c / kRow) * stride + c % kRow * V, vec, o);
       }
-      Elems<T>::store16(rows + (c / kRow) * stride + c % kRow * V, vec, o);
     }
   }
 }
@@ -231,8 +233,8 @@ static int launch_rows(bool write, Kv8RowsParams& p, cudaStream_t st) {
   const int sh = p.c.shift, units = 2 * p.c.heads;
   // items: every sequence's most, or as its rows have it
   const int64_t each = kv8_touched(p.b.max_new, sh), all = kv8_items(p.b.n_tokens, p.b.n_seq, sh);
-  const int64_t items = std::min(each * p.b.n_seq, all);
   p.each = each * p.b.n_seq <= all ? (int)each : 0;
+  const int64_t items = p.each ? each * p.b.n_seq : all + 1;             // (and one more that looks for what the search misses)
   if (items > 0x7fffffff) return fail(kErrLimit, "kv8: too many rows");
   // blocks of threads of `group` threads a unit, each over `per` units while there are blocks enough for every SM
   auto go = [&](auto kern, int group, int64_t an_sm) {

@@ -57,6 +57,22 @@ KV8_HD int kv8_search(int n, int x, First first, Ballot ballot) {
   return lo;
 }
 
+// In a batch whose starts fall the search above misses items of right sequences.  The next of them from item j of sequence s on, which go on
+// behind it (false: none is left).
+template <class SeqOf, class Start, class Ballot>
+KV8_HD bool kv8_next_missed(int n, int shift, SeqOf seq, Start start, Ballot ballot, int& s, int& j, Kv8Item& it) {
+  const auto first = [&](int i) { return kv8_first_item(start(i), i, shift); };
+  for (; s < n; s++, j = 0) {
+    const Kv8Seq q = seq(s);
+    for (;; j++) {
+      it = kv8_item_of(q, j, shift);
+      if (it.n == 0) break;
+      if (kv8_search(n, first(s) + j, first, ballot) != s) { j++; return true; }
+    }
+  }
+  return false;
+}
+
 // The sequence that owns row x (-1: none): found by its start, and where starts that fall mislead the search, the first right one that has it.
 template <class SeqOf, class Start, class Ballot>
 KV8_HD int kv8_owner(int n, int x, SeqOf seq, Start start, Ballot ballot, Kv8Seq& q) {

@@ -188,3 +188,50 @@ def test_broken_starts_leave_the_other_sequences_right_in_several_parts(seqs, G)
             r = slice(c.start_host[s], c.start_host[s] + seqs[s][0])
             assert torch.equal(out[r], outs[0][r]), (change, s)
         assert (out[c.start_host[-1]:] == 7).all()
+
+
+RAGGED = [[(300, 300), (5, 50), (40, 40), (33, 70), (1, 9), (64, 64), (2, 30), (17, 200)], [(700, 900), (1, 1), (3, 64), (0, 20), (2, 65), (9, 9)]]
+
+
+@pytest.mark.parametrize("seqs", RAGGED)
+@pytest.mark.parametrize("block,dt", ((16, "f32"), (64, "bf16"), (128, "f16"), (32, "bf16")))
+def test_broken_starts_leave_the_other_sequences_right_in_ragged_writes_and_reads(seqs, block, dt):
+    from macseek_b200 import _lib, kv8
+    e = enc()
+
+    def make():
+        return R.Case(seqs, 3, 64, block, seed=12, pad=3)
+    c = make()
+    k, v = c.randn(c.rows, 3, 64, dt=dt), c.randn(c.rows, 3, 64, dt=dt)
+    kv8.encode_kv8_write(e, c.cache(), c.batch(), k, v)
+    whole = c
+    rows = [torch.full_like(k, 7), torch.full_like(k, 7)]
+    kv8.encode_kv8_read(e, c.cache(), c.batch(), *rows)
+    e.wait()
+    for change, good in broken_starts(c):
+        c, fresh = make(), make()
+        for i, x in change.items():
+            c.start[i] = x
+        good = [s for s in good if seqs[s][0]]
+        kv8.encode_kv8_write(e, c.cache(), c.batch(), k, v)
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 4
+        mine = torch.zeros(c.k.shape[0], dtype=torch.bool)
+        for s, (n, l) in enumerate(seqs):
+            if s in good:
+                mine[c.table_host[s, :-(-l // block)]] = True
+        mine = mine.cuda()
+        for a, b, f in ((c.k, whole.k, fresh.k), (c.v, whole.v, fresh.v), (c.ks, whole.ks, fresh.ks), (c.vs, whole.vs, fresh.vs)):
+            assert torch.equal(a[mine].nan_to_num(-1) if a.is_floating_point() else a[mine], b[mine].nan_to_num(-1) if b.is_floating_point() else b[mine])
+            assert torch.equal(a[~mine].nan_to_num(-1) if a.is_floating_point() else a[~mine], f[~mine].nan_to_num(-1) if f.is_floating_point() else f[~mine])
+        ko, vo = torch.full_like(k, 7), torch.full_like(k, 7)
+        whole.start.copy_(c.start)
+        kv8.encode_kv8_read(e, whole.cache(), whole.batch(), ko, vo)
+        torch.cuda.synchronize()
+        assert _lib.device_status() == 4
+        keep = torch.zeros(c.rows, dtype=torch.bool)
+        for s in good:
+            keep[c.start_host[s]:c.start_host[s] + seqs[s][0]] = True
+        keep = keep.cuda()
+        for got, want in ((ko, rows[0]), (vo, rows[1])):
+            assert torch.equal(got[keep], want[keep]) and (got[~keep] == 7).all()

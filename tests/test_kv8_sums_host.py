@@ -104,3 +104,43 @@ int main() {
   puts("ok");
 }
 """)
+
+
+def test_every_item_of_a_right_sequence_is_done_once_in_broken_batches(tmp_path):
+    run(tmp_path, BATCH + r"""
+int main() {
+  std::mt19937 rng(9);
+  auto upto = [&](int n) { return (int)(rng() % (unsigned)(n + 1)); };
+  int missed = 0;
+  for (int trial = 0; trial < 2000; trial++) {
+    const bool broken = trial % 4 != 0;
+    const Batch b(upto, broken);
+    const int shift = 4 + upto(3);
+    auto seq = [&](int i) { NEED(i >= 0 && i < b.n_seq); return b.seq(i); };
+    auto start = [&](int i) { NEED(i >= 0 && i <= b.n_seq); return b.start[i]; };
+    auto first = [&](int i) { return kv8_first_item(start(i), i, shift); };
+    std::vector<std::vector<int>> done(b.n_seq);
+    for (int s = 0; s < b.n_seq; s++) done[s].assign(b.seq(s).n, 0);
+    auto work = [&](int s, const Kv8Item& it) {
+      const Kv8Seq q = b.seq(s);
+      NEED(it.row >= q.row && it.row + it.n <= q.row + q.n && it.blk * (1 << shift) + it.at == q.len - q.n + it.row - q.row);
+      for (int r = 0; r < it.n; r++) done[s][it.row - q.row + r]++;
+    };
+    const int64_t items = kv8_items(b.n_tokens, b.n_seq, shift);
+    for (int64_t x = 0; x < items; x++) {
+      const int s = kv8_search(b.n_seq, (int)x, first, Host());
+      const Kv8Item it = kv8_item_of(b.seq(s), (int)x - first(s), shift);
+      if (it.n) work(s, it);
+    }
+    int s = 0, j = 0;
+    Kv8Item it;
+    while (kv8_next_missed(b.n_seq, shift, seq, start, Host(), s, j, it)) { NEED(broken); missed++; work(s, it); }
+    for (auto& d : done) for (int n : d) NEED(n == 1);
+    bool falls = false;                                              // where no start falls nothing is missed, whatever else is wrong
+    for (int i = 0; i < b.n_seq; i++) falls |= b.start[i + 1] < b.start[i];
+    if (!falls) { s = j = 0; NEED(!kv8_next_missed(b.n_seq, shift, seq, start, Host(), s, j, it)); }
+  }
+  NEED(missed > 1000);
+  puts("ok");
+}
+""")
