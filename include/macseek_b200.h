@@ -334,7 +334,7 @@ int msb_kv8_read(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int ele
                  int64_t v_stride, void* stream);
 /* Attention of the batch's rows q ([heads][head_dim] per row, heads a multiple of kv_heads: query head h looks at key head
  * h / (heads / kv_heads)) over the cache, which holds their own tokens already: the row of token p sees the tokens
- * p - window < j <= p (window 0: all up to p) whose blocks are there.
+ * p - window < j <= p (window 0: all up to p) whose blocks are there; blocks that no row sees are not looked at.
  *   out = sum_j exp(l_j) v_j / (sum_j exp(l_j) + exp(sinks[h])),  l_j = scale q . k_j ;  sinks F32[heads] or NULL
  * A row that sees nothing is 0.  Codes must be finite (msb_kv8_write stores no others).  Results do
  * not depend on the run.  scratch: msb_kv8_attn_scratch_bytes(cache, batch, heads) bytes, 16-byte aligned (enough for any

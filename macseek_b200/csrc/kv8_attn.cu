@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
   auto look_up = [&](int i) {
     const int key = k0 + kKdStep * (warp + kKdWarps * (i + (lane >> 1))) + 16 * (lane & 1);
     ids = -1; ksc = 0.f; vex = -INFINITY;
-    if (key < k1) {
+    if (key < k1 && key + 16 > kr.first) {
       ids = i == 0 && kr.lo == 0 ? early_id : __ldg(table + (key >> p.c.shift));
       if (ids < 0 || ids >= p.c.n_blocks) { ids = -1; atomicCAS(p.status, 0, kDevBadBatch); }
       else {

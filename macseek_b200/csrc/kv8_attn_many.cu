@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     constexpr int kNone = -2147483647 - 1;
     auto look_up = [&](int j) {
       const int key = k0 + 2 * kKmKeys * j + 16 * lane;
-      return lane < 2 * kKmKeys / 16 && key < k1 ? __ldg(table + (key >> p.c.shift)) : kNone;
+      return lane < 2 * kKmKeys / 16 && key < k1 && key + 16 > kr.first ? __ldg(table + (key >> p.c.shift)) : kNone;
     };
     // every load is made, from the first block where there is none and of rows behind the last token (which hold anything): without branches
     // between them they leave one after the other.  What is not there becomes zeros when it is put.

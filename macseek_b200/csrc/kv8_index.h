@@ -93,12 +93,16 @@ KV8_HD int kv8_owner(int n, int x, SeqOf seq, Start start, Ballot ballot, Kv8Seq
   return -1;
 }
 
-// Keys that rows [m0, m1) of a sequence look at (row r is token r / G of its new ones): [lo, hi), lo rounded down to `step`.
-struct Kv8Range { int lo, hi; };
+// Keys that rows [m0, m1) of a sequence look at (row r is token r / G of its new ones): [lo, hi), lo being `first` rounded down to `step`.
+// Blocks of 16 tokens before `first` need not be there.
+struct Kv8Range { int lo, hi, first; };
 KV8_HD Kv8Range kv8_range(const Kv8Seq& s, int m0, int m1, int G, int window, int step) {
   const int p0 = s.len - s.n;
-  Kv8Range r{0, p0 + (m1 - 1) / G + 1};
-  if (window && p0 + m0 / G >= window) r.lo = (p0 + m0 / G - window + 1) / step * step;
+  Kv8Range r{0, p0 + (m1 - 1) / G + 1, 0};
+  if (window && p0 + m0 / G >= window) {
+    r.first = p0 + m0 / G - window + 1;
+    r.lo = r.first / step * step;
+  }
   return r;
 }
 // most keys that a tile of `rows` rows looks at, for any sequence

@@ -235,3 +235,22 @@ def test_broken_starts_leave_the_other_sequences_right_in_ragged_writes_and_read
         keep = keep.cuda()
         for got, want in ((ko, rows[0]), (vo, rows[1])):
             assert torch.equal(got[keep], want[keep]) and (got[~keep] == 7).all()
+
+
+@pytest.mark.parametrize("dt", ("f32", "bf16"))
+@pytest.mark.parametrize("seqs,heads,G,window", (([(1, 1000), (3, 500), (1, 90)], 2, 8, 77), ([(1, 4000)], 8, 8, 1500), ([(90, 700), (200, 900)], 4, 8, 100),
+                                                 ([(600, 2000)], 4, 8, 1000), ([(64, 300)], 1, 16, 1)))
+def test_blocks_before_the_window_need_not_be_there(seqs, heads, G, window, dt):
+    """A program with a sliding window gives blocks back that no row sees any more; their ids in the table are anything then."""
+    from macseek_b200 import kv8
+    for dim in (64, 128):
+        c = R.Case(seqs, heads, dim, 16, seed=13, pad=1)
+        for s, (n, l) in enumerate(seqs):
+            gone = max(0, l - n - window + 1) // 16
+            c.table[s, :gone] = torch.tensor([-1, 2 ** 31 - 1, c.k.shape[0]], dtype=torch.int32, device="cuda").repeat(gone)[:gone]
+        cache, batch, e = c.cache(), c.batch(), enc()
+        q = c.randn(c.rows, heads * G, dim, dt=dt, mul=3.0)
+        out = torch.full_like(q, 7)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, heads * G), window=window)
+        e.wait()                                                     # raises where the batch is called broken
+        check_attn(c, q, out, torch.full_like(q, 7), dim ** -0.5, window, None)
