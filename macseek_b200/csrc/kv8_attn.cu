@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kKdWarps * 32, kd_blocks(sizeof(T) == 4, D)) k
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 120);
+    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 120);
     const float inv = kv8_pow2(-e);
     qs[h] = kv8_pow2(e) * p.scale * kLog2e;
 #pragma unroll

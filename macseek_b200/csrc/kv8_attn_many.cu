@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
           for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -60), 120);
+          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 120);
           const float inv = p.scale < 0.f ? -kv8_pow2(-e) : kv8_pow2(-e);
           if (c == 0) hd->f0[t * 128 + (warp & 3) * 32 + r] = kv8_pow2(e) * fabsf(p.scale) * kLog2e;
           uint32_t hi[4], lo[4];

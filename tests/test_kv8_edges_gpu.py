@@ -254,3 +254,19 @@ def test_blocks_before_the_window_need_not_be_there(seqs, heads, G, window, dt):
         kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, heads * G), window=window)
         e.wait()                                                     # raises where the batch is called broken
         check_attn(c, q, out, torch.full_like(q, 7), dim ** -0.5, window, None)
+
+
+@pytest.mark.parametrize("dt", ("f32", "bf16"))
+@pytest.mark.parametrize("n", (1, 600, 1000))
+def test_attention_of_tiny_queries_under_a_large_scale(n, dt):
+    """Queries near the smallest numbers and a scale that makes ordinary logits of them."""
+    from macseek_b200 import kv8
+    c = R.Case([(n, 1100)], 4, 64, 16, seed=15)
+    cache, batch, e = c.cache(), c.batch(), enc()
+    base = c.randn(c.rows, 32, 64, dt=dt)
+    for ex in (40, 60, 70, 90, 110):
+        q = base * 2.0 ** -ex
+        out = torch.zeros_like(q)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 32), scale=2.0 ** (ex - 3))
+        e.wait()
+        check_attn(c, q, out, torch.zeros_like(out), 2.0 ** (ex - 3), 0, None)
