@@ -10,7 +10,7 @@
 //   F32 rows  queries and weights are two halves each: one row tile, and twice the products
 //   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32, F32: its second halves in the others), O from 128 on; F32: the
 //             products of the second halves have a sum of their own from 384 on
-//   sums      the tensor core cuts off what a sum does not hold, so O is added to a sum elsewhere and begun anew every 512 keys (F32: tensor memory
+//   sums      the tensor core cuts off what a sum does not hold, so O is added to a sum elsewhere and begun anew every 1024 keys (F32: tensor memory
 //             from 256 on) or 16384 (16 bits: the scratch), and F32 scores begin with the queries' second halves.  200K tokens with values
 //             of one sign, error without: 1.1e-3
 // Bound by the exponentials (16 a clock beside those on the multiply-add pipe) and by shared memory: the products read 48 KB a tile and row
@@ -435,10 +435,10 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
             const int hi = cut ? last - base - 16 * c : 16, lo = cut ? first - base - 16 * c : 0;
 #pragma unroll
             for (int i = 0; i < 16; i++)
-              if (i <= hi && i >= lo) top = fmaxf(top, fmaf(__uint_as_float(a[i]), f, sc.y));
+              if (i <= hi && i >= lo) top = fmaxf(top, __fmaf_rd(__uint_as_float(a[i]), f, sc.y));
             __syncwarp();
           }
-          if (m == -INFINITY) m = floorf(top) - kKmFirst;
+          if (m == -INFINITY) m = __fadd_rd(floorf(top), -kKmFirst);
           mm = m == -INFINITY ? 0.f : m;
         }
         // ---- weights.  The reference begins 7 below the first tile's largest exponent and stays unless the weights of 16 keys sum to more than
@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
         // A half holds nothing below 2^-25, so N keys lose N 2^-31 at most beside the largest; the second halves of F32 weights, taken times
         // 2^11, hold what is 2^11 below
         bool lost = false;
+        constexpr int kTries = 4;
         int tries = 0;
         uint32_t w[4][16];
         float part[4];
@@ -459,7 +460,8 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
 #pragma unroll
           for (int h = 0; h < 4; h++) {
             const float4 sc = hd->sc[s][h];
-            const uint64_t f = kv8_two(f0 * sc.x, f0 * sc.x), b = kv8_two(sc.y - mm, sc.y - mm);
+            const float off = __fadd_ru(sc.y, -mm);
+            const uint64_t f = kv8_two(f0 * sc.x, f0 * sc.x), b = kv8_two(off, off);
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
               float x, y;
@@ -467,11 +469,15 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
               w[h][i] = __float_as_uint(x); w[h][i + 1] = __float_as_uint(y);
             }
           }
-          if (cut) {
-            const int hi = last - base, lo = first - base;
+          if (cut || tries == kTries) {
+            const int hi = cut ? last - base : 64, lo = cut ? first - base : 0;
+            const float most = tries == kTries && !lost ? 15.f : INFINITY;
 #pragma unroll
-            for (int i = 0; i < 64; i++)
-              if (i > hi || i < lo) w[i >> 4][i & 15] = 0xFF800000u;
+            for (int i = 0; i < 64; i++) {
+              float x;
+              asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(__uint_as_float(w[i >> 4][i & 15])), "f"(most));
+              w[i >> 4][i & 15] = i > hi || i < lo ? 0xFF800000u : __float_as_uint(x);
+            }
             __syncwarp();
           }
 #pragma unroll
@@ -490,10 +496,11 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
             part[h] = y + z;
           }
           const float most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-          if (!__any_sync(0xffffffffu, most > 60000.f && !lost)) break;
+          if (tries == kTries || !__any_sync(0xffffffffu, most > 60000.f && !lost)) break;
           // by the next power of two above the sum, or, where that is beyond 32 bits or near the end of km_exp2_fma's range (which a sum then
-          // does not show to be passed), to the largest exponent.  A row whose products are infinite has none, and beyond 2^35 exponents are
-          // too coarse for one: after four times its weights stay what they are
+          // does not show to be passed), to the largest exponent.  A row whose products are infinite has none.  The reference is a whole number;
+          // beyond 2^27 not every one is held, and it is the next one down (weights come out larger, never smaller), and after four times weights
+          // that are still too large become 2^15, all of them: their logits differ by less than a step of 32 bits
           constexpr float kFar = 100.f;
           float up = most > 256.f && !lost ? (float)((int)(__float_as_uint(most) >> 23) - 126) - kKmFirst : 0.f;
           if (__any_sync(0xffffffffu, up > kFar)) {
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
 #pragma unroll
               for (int i = 0; i < 16; i++) {
                 const int key = base + 16 * k + i;
-                if (!cut || (key >= first && key <= last)) top = fmaxf(top, fmaf(__uint_as_float(w[0][i]), f0 * sc.x, sc.y - mm));
+                if (!cut || (key >= first && key <= last)) top = fmaxf(top, __fmaf_rd(__uint_as_float(w[0][i]), f0 * sc.x, __fadd_ru(sc.y, -mm)));
               }
               __syncwarp();
             }
@@ -515,9 +522,10 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
               up = lost ? 0.f : ceilf(top) - kKmFirst;
             }
           }
-          if (++tries == 4) lost = true;
-          const float f = km_exp2(-up);
-          m += up; mm = m; l *= f;
+          tries++;
+          const float moved = up > 0.f ? __fadd_rd(m, up) : m, f = moved > m ? km_exp2(m - moved) : 1.f;
+          if (moved > m) m = mm = moved;
+          l *= f;
           if (j) {                                       // the products of the tile before are there (those of two before are: this tile's scores are)
             ok = wait(&hd->odone[t], j - 1, kDevWaitFull);
             if (!ok) break;

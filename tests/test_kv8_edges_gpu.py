@@ -270,3 +270,30 @@ def test_attention_of_tiny_queries_under_a_large_scale(n, dt):
         kv8.encode_kv8_attn(e, cache, batch, q, out, kv8.attn_scratch(cache, batch, 32), scale=2.0 ** (ex - 3))
         e.wait()
         check_attn(c, q, out, torch.zeros_like(out), 2.0 ** (ex - 3), 0, None)
+
+
+@pytest.mark.parametrize("dt", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("n", (1, 600, 1000))
+@pytest.mark.parametrize("sign", (1.0, -1.0))
+def test_attention_over_logits_beyond_the_steps_of_32_bits(n, dt, sign):
+    """Logits of 2^20 to 2^60, whose last bits are larger than an exponent: the largest key's value is the result, wherever it lies."""
+    from macseek_b200 import kv8
+    G, dim = 8, 64
+    c = R.Case([(n, 1100)], 4, dim, 16, seed=14)
+    c.ks.fill_(1)
+    cache, batch, e = c.cache(), c.batch(), enc()
+    scratch = kv8.attn_scratch(cache, batch, 4 * G)
+    q = torch.zeros(c.rows, 4 * G, dim, dtype=R.DT[dt], device="cuda")
+    q[:, :, 3] = torch.linspace(1, 1.9375, 16, device="cuda").repeat(2).to(q.dtype)
+    for ex in (20, 24, 26, 27, 28, 29, 30, 31, 32, 34, 36, 40, 60):
+        for at in (5, 70, 333):
+            c.k.fill_(0)
+            c.k[:, :, :, 3] = 0x70 if sign > 0 else 0x78             # 128, 256
+            c.k[c.table_host[0, at // 16], :, at % 16, 3] = 0x78 if sign > 0 else 0x70
+            out = torch.zeros_like(q)
+            kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, scale=sign * 2.0 ** (ex - 8))
+            e.wait()
+            v = c.held(0, "v")[:, at].repeat_interleave(G, 0)
+            sees = torch.arange(1100 - n, 1100, device="cuda")[:, None, None] >= at
+            bad = sees & ((out.double() - v[None]).abs() > v.abs() * (2.0 ** -11 + 2.0 ** -20 + R.half_step(q.dtype)[0]) + 2.0 ** -30)
+            assert not (bad | out.isnan()).any(), (ex, at, int(bad.sum()), out.isnan().sum())
