@@ -165,6 +165,8 @@ int head_norm_rope(int elem_type, const void* q, int q_heads, int64_t q_stride, 
   if (rot < 0 || rot % 2 || first < 0 || rot > D || first > D - rot || first % 8 || rot % (halves ? 16 : 8))
     return fail(kErrArg, "%s: rotation of %d dims from %d on (first a multiple of 8, the count of 8, by halves of 16)", what, rot, first);
   if (!pos || n_pos <= 0 || (rot && !cs)) return fail(kErrArg, "%s: null pointer or no positions", what);
+  if ((reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(cs) | reinterpret_cast<uintptr_t>(q_w) | reinterpret_cast<uintptr_t>(k_w)) & 3)
+    return fail(kErrArg, "%s: positions, factors or gains are not aligned to their elements", what);
   NormRopeParams p{};
   bool v[4] = {true, true, true, true};
   int rc;

@@ -575,6 +575,7 @@ int kv8_attn(const msb_kv8_cache* c, const msb_kv8_batch* b, int elem_type, cons
   bool qv, ov;
   if ((rc = kv8_rows_check(q, q_stride, heads, c->head_dim, elem_type, what, &qv))) return rc;
   if ((rc = kv8_rows_check(out, out_stride, heads, c->head_dim, elem_type, what, &ov))) return rc;
+  if (reinterpret_cast<uintptr_t>(sinks) & 3) return fail(kErrArg, "%s: sinks are not aligned to F32", what);
   if (window < 0) return fail(kErrArg, "%s: window %d", what, window);
   if (!(scale == scale) || scale - scale != 0.f) return fail(kErrArg, "%s: scale is not a number", what);
   int dev, sms;

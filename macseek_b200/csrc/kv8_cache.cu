@@ -19,12 +19,15 @@ int kv8_check(const msb_kv8_cache* c, const msb_kv8_batch* b, const char* what, 
     return fail(kErrArg, "%s: %d tokens in a block (16, 32, 64 or 128)", what, c->block);
   if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(kErrArg, "%s: null pointer in the cache", what);
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return fail(kErrArg, "%s: codes must be 16-byte aligned", what);
+  if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 3) return fail(kErrArg, "%s: scales are not aligned to F32", what);
   if (b->n_seq <= 0 || b->n_seq > 65535) return fail(kErrArg, "%s: %d sequences (1 to 65535)", what, b->n_seq);
   if (b->n_tokens <= 0 || b->max_new <= 0 || b->max_new > b->n_tokens) return fail(kErrArg, "%s: %d rows, at most %d new ones", what, b->n_tokens, b->max_new);
   if (b->max_len < b->max_new || b->max_len > (1 << 30)) return fail(kErrArg, "%s: at most %d tokens, %d of them new", what, b->max_len, b->max_new);
   if (b->table_stride <= 0 || (int64_t)b->table_stride * c->block < b->max_len)
     return fail(kErrArg, "%s: %d blocks of %d tokens do not hold %d", what, b->table_stride, c->block, b->max_len);
   if (!b->seq_start || !b->kv_len || !b->table) return fail(kErrArg, "%s: null pointer in the batch", what);
+  if ((reinterpret_cast<uintptr_t>(b->seq_start) | reinterpret_cast<uintptr_t>(b->kv_len) | reinterpret_cast<uintptr_t>(b->table)) & 3)
+    return fail(kErrArg, "%s: the batch's arrays are not aligned to int32", what);
   int shift = 4;
   while ((1 << shift) < c->block) shift++;
   *cc = Kv8Cache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, c->n_blocks, c->kv_heads, shift};
