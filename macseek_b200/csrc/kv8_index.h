@@ -119,6 +119,8 @@ constexpr int kKv8FewRows = 16, kKv8FewStep = 32, kKv8ManyRows = 256, kKv8ManyRo
 // Keys whose products a tensor core adds up by itself, cutting off up to 2^-23 of the sum at every 16 keys: in a block of few rows (a part at
 // most; a warp has a quarter of them, and of F32 rows it begins anew) and in one of many (then the sum is begun anew).
 constexpr int kKv8FewKeys = 65536, kKv8Fold = 16384, kKv8FoldF32 = 1024;
+// parts that this takes for few rows (256 at most, 16M tokens: a bound that no sequence comes near shall not cost a scratch and blocks for it)
+inline int kv8_least(int keys) { const int n = (int)((keys + kKv8FewKeys - 1ll) / kKv8FewKeys); return n < 256 ? n : 256; }
 
 // splits at most of either kernel, whatever the window
 struct Kv8Most { int few, many; };
@@ -127,7 +129,7 @@ inline Kv8Most kv8_most(int n_seq, int max_new, int max_len, int kv_heads, int h
   const int64_t few = 3ll * sms * (n_seq > 1 ? 6 : 1) / ((rows + kKv8FewRows - 1) / kKv8FewRows * groups);
   const int many_rows = f32 ? kKv8ManyRowsF32 : kKv8ManyRows;
   const int64_t many = 4ll * sms / ((rows + many_rows - 1) / many_rows * groups);
-  const int64_t least = (max_len + kKv8FewKeys - 1ll) / kKv8FewKeys;
+  const int64_t least = kv8_least(max_len);
   return Kv8Most{(int)(few < least ? least : few < full ? few : full), (int)(many < 1 ? 1 : many < full ? many : full)};
 }
 inline Kv8Plan kv8_plan(int n_seq, int max_new, int max_len, int kv_heads, int heads, int dim, bool f32, int window, int sms) {
@@ -145,7 +147,7 @@ inline Kv8Plan kv8_plan(int n_seq, int max_new, int max_len, int kv_heads, int h
     const int64_t units = pl.tiles * groups, room = k ? 1 : f32 && dim == 128 ? 2 : 3;      // blocks an SM at once
     // few: keys of 16 rows that an SM does in a us, by all its blocks (one alone: 1 / 1.7 of them); many: us a key of a block's rows
     const double speed = f32 ? (dim == 64 ? 182 : 115) : (dim == 64 ? 230 : 155), per_key = f32 ? (dim == 64 ? 0.032 : 0.044) : (dim == 64 ? 0.031 : 0.034);
-    for (int n = k ? 1 : (int)up(span, kKv8FewKeys), last = 0; n <= top; n = n < top ? kv8_min(top, n + kv8_max(1, n / 8)) : top + 1) {
+    for (int n = k ? 1 : kv8_least(span), last = 0; n <= top; n = n < top ? kv8_min(top, n + kv8_max(1, n / 8)) : top + 1) {
       const int chunk = kv8_max((int)(up(up(span, n), unit) * unit), kKv8Least), parts = (int)up(span, chunk);
       if (parts == last) continue;
       last = parts;

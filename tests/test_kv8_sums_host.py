@@ -34,7 +34,8 @@ int main() {
     if ((int64_t)p.chunk * p.splits < span) { puts("keys"); return 1; }
     if (!p.many) {
       few++;
-      if (p.chunk > kKv8FewKeys) { printf("%d keys in a part\n", p.chunk); return 1; }
+      if (p.chunk > kKv8FewKeys && (span <= 256 * kKv8FewKeys || p.chunk > span / 256 + 64)) { printf("%d keys in a part\n", p.chunk); return 1; }
+      if (p.splits > 256 && p.splits > 3 * 148 * 6) { printf("%d parts\n", p.splits); return 1; }
     }
   }
   if (few < 1000) { puts("too few cases"); return 1; }
