@@ -325,7 +325,8 @@ typedef struct {
  * (50 where none is) and, where the block holds older tokens, at least its E so far; those are then rounded again to the
  * larger scale.  Codes are rounded to nearest even; what lies beyond becomes +-448 * 2^E, an infinity too, which does not
  * count for the maximum; a NaN becomes 0 and sets device status 5.  A block whose first token is new starts over, whatever it held.  Rows of a block behind the sequence's
- * last token keep their bytes and mean nothing.  No two sequences of a call may write to one block. */
+ * last token keep their bytes and mean nothing.  No block may be written to twice in a call, by two sequences or by one whose
+ * table names it twice. */
 int msb_kv8_write(const msb_kv8_cache* cache, const msb_kv8_batch* batch, int elem_type, const void* k, const void* v,
                   int64_t k_stride, int64_t v_stride, void* stream);
 /* The values of the batch's rows (the last seq_start[s + 1] - seq_start[s] tokens of each sequence) into k, v; zeros for a

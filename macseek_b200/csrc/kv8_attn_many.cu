@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     const bool leader = elect_one();
     const uint64_t q_d = ts_desc(smem_u32(qs_mem)), k_d = ts_desc(smem_u32(kmem)), v_d = km_desc_mn(smem_u32(vmem), kKmKeys * 128);
     bool ok = wait(&hd->qfull, 0, kDevWaitFull);
-    // round j: the scores of tile j + 1, then the output's products of tile j (one copy of the code: it has to stay in the instruction cache)
+    // round j: the scores of tile j + 1, then the output's products of tile j (the loops stay rolled: unrolled weights made the prompt three times
+    // as long)
 #pragma unroll 1
     for (int j = -1; ok && j < n; j++) {
       if (j + 1 < n) {
@@ -405,7 +406,8 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
     for (int j0 = 0, j1; ok && j0 < n; j0 = j1) {
       j1 = FOLD ? min(n, j0 + S::kFold) : n;
       if (FOLD && j0) {
-        ok = wait(&hd->odone[t], j0 - 1, kDevWaitFull);
+        // (the scores of this tile first: with them the products of two tiles ago are there, and the phase waited for is the next)
+        ok = wait(&hd->sfull[t][j0 & 1], j0 >> 1, kDevWaitFull) && wait(&hd->odone[t], j0 - 1, kDevWaitFull);
         if (!ok) break;
         __syncwarp();
         ts_fence_after();

@@ -92,10 +92,6 @@ def _rows(name, t, n_tokens, heads, dim, device):
     return ty
 
 
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
-
-
 _WRITE, _READ, _ATTN = (_lib.address(f) for f in (_lib.lib.msb_kv8_write, _lib.lib.msb_kv8_read, _lib.lib.msb_kv8_attn))
 
 

@@ -297,3 +297,21 @@ def test_attention_over_logits_beyond_the_steps_of_32_bits(n, dt, sign):
             sees = torch.arange(1100 - n, 1100, device="cuda")[:, None, None] >= at
             bad = sees & ((out.double() - v[None]).abs() > v.abs() * (2.0 ** -11 + 2.0 ** -20 + R.half_step(q.dtype)[0]) + 2.0 ** -30)
             assert not (bad | out.isnan()).any(), (ex, at, int(bad.sum()), out.isnan().sum())
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("dim", (64, 128))
+def test_attention_whose_sums_begin_anew_under_peaked_weights(seed, dim):
+    """F32 rows over a little more than 1024 keys, a few of which have nearly all the weight: what O held is taken when all of it is there."""
+    from macseek_b200 import kv8
+    seqs = [(151, 151), (24, 50), (191, 897 + 300 * (seed % 2)), (200, 1107), (77, 77), (271, 2580)]
+    c = R.Case(seqs, 3, dim, 16, seed=seed, pad=1)
+    cache, batch, e = c.cache(), c.batch(), enc()
+    q = c.randn(c.rows, 6, dim, mul=10.0 if seed < 3 else 3.0)
+    sinks = c.randn(6, mul=3.0)
+    scratch = kv8.attn_scratch(cache, batch, 6)
+    for _ in range(3):
+        out = torch.full_like(q, 7)
+        kv8.encode_kv8_attn(e, cache, batch, q, out, scratch, sinks=sinks)
+        e.wait()
+        check_attn(c, q, out, torch.full_like(q, 7), dim ** -0.5, 0, sinks)
