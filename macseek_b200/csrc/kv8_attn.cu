@@ -77,7 +77,7 @@ __device__ __forceinline__ float4 kd_load4_of(uint32_t addr) {
   return v;
 }
 
-// Blocks of an SM: F32 rows of 128 dims need more registers than a third of an SM's threads have (64 ragged sequences: 147 us with two blocks,
+// Blocks of an SM: F32 rows of 128 dims need more registers than a third of an SM's threads have (64 ragged sequences: 150 us with two blocks,
 // 211 with three and 270 bytes a thread in local memory).  Four of 64 dims gain nothing (200K tokens, bf16: 44 us with three).
 constexpr int kd_blocks(bool f32, int dim) { return f32 && dim == 128 ? 2 : 3; }
 // CLUSTER: the parts of a row are the blocks of a cluster, which join them through one another's shared memory

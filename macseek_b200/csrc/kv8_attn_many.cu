@@ -6,7 +6,7 @@
 //   warps     0..3, 4..7 a row tile of 128 each: a thread has a row, computes its weights and, when their reference moves, rescales O;
 //             then four that convert keys and values, four buffers each; then one that issues the products
 //   S         has two buffers a row tile: the scores of a tile are there before the weights of the one before are done.  (One buffer of 128
-//             keys reads the queries half as often: 375 us for the prompt below, but 107 for the chunks.)
+//             keys reads the queries half as often: 375 us for the prompt below and 107 for the chunks, when two were 403 and 98.)
 //   F32 rows  queries and weights are two halves each: one row tile, and twice the products
 //   TMEM      [256 t, ..): S of row tile t twice (64 columns; P in the first 32, F32: its second halves in the others), O from 128 on; F32: the
 //             products of the second halves have a sum of their own from 384 on
@@ -14,8 +14,8 @@
 //             from 256 on) or 16384 (16 bits: the scratch), and F32 scores begin with the queries' second halves.  200K tokens with values
 //             of one sign, error without: 1.1e-3
 // Bound by the exponentials (16 a clock beside those on the multiply-add pipe) and by shared memory: the products read 48 KB a tile and row
-// tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 403 us = 683 TFLOP/s, of which an eighth goes into a block's
-// start and end; ragged chunks of up to 333 tokens, 32 heads over 4 of 64, behind up to 8192: 98 us.  Every wait is bounded.
+// tile, the conversion writes 32 KB.  4096 tokens, 64 heads over 8 of 128, bf16: 407 us = 675 TFLOP/s, of which an eighth goes into a block's
+// start and end; ragged chunks of up to 333 tokens, 32 heads over 4 of 64, behind up to 8192: 92 us.  Every wait is bounded.
 #include <algorithm>
 #include "kv8_attn.cuh"
 #include "ts_gemm.cuh"
@@ -130,7 +130,7 @@ __device__ __noinline__ void km_fold(uint32_t o, uint32_t column, float* place, 
   *kept = make_float2(m, first ? l : fmaf(kept->y, f, l));
 }
 
-// FOLD: parts may have more than kFold tiles (a prompt of 4096 tokens, bf16: 403 us without the call in its loop, 411 with it)
+// FOLD: parts may have more than kFold tiles (a prompt of 4096 tokens, bf16: 403 us without it, 411 with it; a chunk of 512 behind 200K 2 %)
 template <class T, int D, bool FOLD>
 __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_kernel(const Kv8AttnParams p) {
   using S = KmShape<T, D>;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(KmShape<T, D>::kWarps * 32, 1) kv8_attn_many_k
         // ---- weights.  The reference begins 7 below the first tile's largest exponent and stays unless the weights of 16 keys sum to more than
         // 60000 (a half holds each of them below that).  Then those of the warp's rows that sum to more than 2^8 move up by a whole number, to a
         // sum of 2^6 to 2^7, what has been summed against the old reference is scaled, and the weights are made again.  (Were only the row
-        // above 60000 moved, a prompt of 4096 tokens would take about 420 us instead of 403.)
+        // above 60000 moved, a prompt of 4096 tokens takes 4 % longer.)
         // A half holds nothing below 2^-25, so N keys lose N 2^-31 at most beside the largest; the second halves of F32 weights, taken times
         // 2^11, hold what is 2^11 below
         bool lost = false;
